@@ -48,6 +48,22 @@ SIGNATURES = {
     "b200w4a4_map_cache_stats": (None, [POINTER(ctypes.c_ulonglong), POINTER(ctypes.c_ulonglong)]),
 }
 
+# the same for include/b200w4a4_decoder.h
+_LL = ctypes.c_longlong
+DECODER_SIGNATURES = {
+    "b200w4a4_rms_norm_quant": (c_int, [c_void_p, c_int, _LL, c_void_p, _LL, c_void_p, c_int, c_float, c_void_p, c_int,
+                                        c_void_p, c_void_p, c_int, c_int, c_float, c_void_p]),
+    "b200w4a4_quantize_weight_grouped": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
+    "b200w4a4_linear_w4_group": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                                         c_int, c_int, c_int, c_void_p]),
+    "b200w4a4_rotary": (c_int, [c_void_p, _LL, _LL, c_void_p, _LL, _LL, c_int, c_void_p, _LL, _LL, c_void_p, _LL, _LL, c_int,
+                                c_int, c_void_p, _LL, c_void_p, c_int, _LL, c_int, c_int, c_int, c_int, c_void_p]),
+    "b200w4a4_window_attention_workspace_bytes": (c_size_t, [c_int] * 8),
+    "b200w4a4_window_attention": (c_int, [c_void_p, _LL, _LL, _LL, c_void_p, _LL, _LL, _LL, c_void_p, _LL, _LL, _LL, c_void_p,
+                                          c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                          c_float, c_void_p, c_size_t, c_void_p]),
+}
+
 _LIB: Optional[ctypes.CDLL] = None
 _LOAD_ERROR: Optional[BaseException] = None
 _LOCK = threading.Lock()
@@ -82,7 +98,7 @@ def load() -> ctypes.CDLL:
                     raise RuntimeError(f"{path} is missing or older than its sources and nvcc was not found")
                 path = _build.build()
             lib = ctypes.CDLL(str(path))
-            for name, (res, args) in SIGNATURES.items():
+            for name, (res, args) in {**SIGNATURES, **DECODER_SIGNATURES}.items():
                 fn = getattr(lib, name)
                 fn.restype = res
                 fn.argtypes = args

@@ -15,6 +15,7 @@
 
 #include "../../include/b200w4a4.h"
 #include "attn_glue.cuh"
+#include "device_state.cuh"
 #include "gemm_w4a4.cuh"
 #include "quant_act.cuh"
 #include "weight_pack.cuh"
@@ -344,6 +345,14 @@ int noalloc_scratch(uint8_t** base) {
 }
 
 }  // namespace
+
+int b200w4a4::current_device(int* sm_count, int** status) {
+  DeviceState* st = nullptr;
+  const int rc = device_state(&st);
+  if (rc == B200W4A4_OK && sm_count != nullptr) *sm_count = st->sm_count;
+  if (rc == B200W4A4_OK && status != nullptr) *status = st->status_ptr;
+  return rc;
+}
 
 extern "C" {
 

@@ -16,12 +16,13 @@ from pathlib import Path
 CSRC = Path(__file__).resolve().parent
 ROOT = CSRC.parent.parent
 LIB_NAME = "libb200w4a4.so"
-SOURCES = ["b200w4a4_api.cu"]
-HEADERS = ["gemm_w4a4.cuh", "quant_act.cuh", "weight_pack.cuh", "ptx.cuh", "attn_glue.cuh"]
+SOURCES = ["b200w4a4_api.cu", "decoder_api.cu"]
+HEADERS = ["gemm_w4a4.cuh", "quant_act.cuh", "weight_pack.cuh", "ptx.cuh", "attn_glue.cuh", "device_state.cuh",
+           "rms_norm.cuh", "rotary.cuh", "w4_group.cuh", "window_attn.cuh"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
-    "-shared", "-Xcompiler", "-fPIC",
+    "-shared", "-Xcompiler", "-fPIC", "--threads", "0",
 ]
 
 
@@ -44,7 +45,7 @@ def is_stale(lib: Path) -> bool:
     if not lib.exists():
         return True
     t = lib.stat().st_mtime
-    deps = [CSRC / s for s in SOURCES + HEADERS] + [ROOT / "include" / "b200w4a4.h"]
+    deps = [CSRC / s for s in SOURCES + HEADERS] + [ROOT / "include" / h for h in ("b200w4a4.h", "b200w4a4_decoder.h")]
     return any(d.stat().st_mtime > t for d in deps if d.exists())
 
 

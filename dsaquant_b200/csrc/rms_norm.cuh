@@ -1,0 +1,255 @@
+// Residual addition, RMSNorm and per-token 8-bit codes in one pass over a row:
+//   s     = x + residual                        (fp32; residual_out = s rounded to x's type)
+//   y     = s * rsqrt(mean(s^2) + eps) * weight (fp32; the norm reads s before its rounding)
+//   scale = max(max|y|, 1e-5) / top * clip      top = 127 (int8) or 448 (e4m3)
+//   code  = clamp(rint(y / scale), -128, 127)   or  y / scale rounded to e4m3, saturating
+// The row is loaded once and stays in registers as fp32 through both reductions (sum of squares,
+// abs-max), so what moves is x, the residual in and out, one byte a value and four a row.
+//
+// A row whose sum of squares or whose y is not finite has no meaningful codes: its scale is NaN
+// (whatever is computed from it shows it) and its codes are 0.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "quant_act.cuh"  // Chunk, row_reduce
+
+namespace b200w4a4 {
+
+enum : int { CODES_INT8 = 0, CODES_E4M3 = 1 };
+
+struct RmsNormArgs {
+  const void* x;         // [M, D], row pitch x_ld elements
+  const void* residual;  // same type, row pitch r_ld, or null
+  const void* weight;    // [D] of type w_dtype
+  void* codes;           // [M, D] bytes
+  float* scale;          // [M]
+  void* residual_out;    // [M, D] of x's type, or null with residual
+  long long x_ld, r_ld;
+  float eps, clip;
+  int w_dtype, format, M, D;
+};
+
+namespace detail {
+
+__device__ __forceinline__ float load_f32(const __half* p) { return __half2float(*p); }
+__device__ __forceinline__ float load_f32(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ float load_f32(const float* p) { return *p; }
+__device__ __forceinline__ void store_f32(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void store_f32(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void store_f32(float* p, float v) { *p = v; }
+
+// Eight values stored in x's type with one or two 128-bit stores.
+__device__ __forceinline__ void store8(__half* p, const float (&v)[8]) {
+  __half2 h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+  *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
+  __nv_bfloat162 h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+  *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
+}
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+
+// Eight weights; the weight vector is shared by every row, so it goes through the read-only cache.
+template <typename W>
+__device__ __forceinline__ void weight8(const W* p, float (&w)[8]) {
+  if constexpr (sizeof(W) == 4) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+    w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+  } else {
+    Chunk<W> c;
+    c.raw = __ldg(reinterpret_cast<const uint4*>(p));
+    c.values(w);
+  }
+}
+
+// max that keeps a NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t code_int8(float y, float inv) {
+  return __float_as_uint(fminf(fmaxf(y * inv, -128.0f), 127.0f) + kRoundMagic);  // low byte
+}
+__device__ __forceinline__ uint32_t code_e4m3x2(float lo, float hi, float inv) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(lo * inv, hi * inv), __NV_SATFINITE, __NV_E4M3);
+}
+
+}  // namespace detail
+
+// TPR threads share a row and hold NCH * 8 of its values each.  VEC: eight consecutive values a
+// chunk, moved with 128-bit accesses (D, pitches and addresses allow it).  Otherwise a chunk is
+// eight values TPR apart and every access moves one value, coalesced across the threads.
+template <typename T, int TPR, int NCH, bool VEC>
+__global__ void __launch_bounds__(256) rms_norm_quant_kernel(const RmsNormArgs a) {
+  constexpr int ROWS = 256 / TPR;
+  __shared__ float red[2][8];
+  const int sub = threadIdx.x / TPR;
+  const int t = threadIdx.x % TPR;
+  const long long row = static_cast<long long>(blockIdx.x) * ROWS + sub;
+  const bool row_ok = row < a.M;
+  const T* xr = static_cast<const T*>(a.x) + (row_ok ? row : 0) * a.x_ld;
+  const T* rr = static_cast<const T*>(a.residual);
+  if (rr != nullptr) rr += (row_ok ? row : 0) * a.r_ld;
+  T* ro = static_cast<T*>(a.residual_out) + row * a.D;
+  auto at = [&](int i, int e) { return VEC ? 8 * (t + i * TPR) + e : (8 * i + e) * TPR + t; };
+
+  float v[NCH][8];
+  float ss = 0.0f;
+  if constexpr (VEC) {
+    detail::Chunk<T> cx[NCH], cr[NCH];
+#pragma unroll
+    for (int i = 0; i < NCH; ++i)
+      if (row_ok && at(i, 0) < a.D) cx[i].load(xr + at(i, 0));
+    if (rr != nullptr) {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i)
+        if (row_ok && at(i, 0) < a.D) cr[i].load(rr + at(i, 0));
+    }
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      if (row_ok && at(i, 0) < a.D) {
+        cx[i].values(v[i]);
+        if (rr != nullptr) {
+          float r[8];
+          cr[i].values(r);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[i][e] += r[e];
+          detail::store8(ro + at(i, 0), v[i]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = 0.0f;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NCH; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] = row_ok && at(i, e) < a.D ? detail::load_f32(xr + at(i, e)) : 0.0f;
+    if (rr != nullptr && row_ok) {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (at(i, e) < a.D) {
+            v[i][e] += detail::load_f32(rr + at(i, e));
+            detail::store_f32(ro + at(i, e), v[i][e]);
+          }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NCH; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss = fmaf(v[i][e], v[i][e], ss);
+  ss = row_reduce<TPR, false>(ss, red[0], sub);
+  const float rstd = rsqrtf(ss / static_cast<float>(a.D) + a.eps);
+
+  float amax = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    float w[8];
+    if constexpr (VEC) {
+      if (at(i, 0) < a.D) {
+        if (a.w_dtype == XDT_F16) detail::weight8(static_cast<const __half*>(a.weight) + at(i, 0), w);
+        else if (a.w_dtype == XDT_BF16) detail::weight8(static_cast<const __nv_bfloat16*>(a.weight) + at(i, 0), w);
+        else detail::weight8(static_cast<const float*>(a.weight) + at(i, 0), w);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = 0.0f;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = at(i, e);
+        w[e] = 0.0f;
+        if (c < a.D) {
+          if (a.w_dtype == XDT_F16) w[e] = detail::load_f32(static_cast<const __half*>(a.weight) + c);
+          else if (a.w_dtype == XDT_BF16) w[e] = detail::load_f32(static_cast<const __nv_bfloat16*>(a.weight) + c);
+          else w[e] = detail::load_f32(static_cast<const float*>(a.weight) + c);
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[i][e] = v[i][e] * rstd * w[e];
+      amax = detail::max_nan(amax, fabsf(v[i][e]));
+    }
+  }
+  // a NaN must survive the reduction too: it travels as +inf, which no finite row reaches
+  if (!(amax < INFINITY)) amax = INFINITY;
+  amax = row_reduce<TPR, true>(amax, red[1], sub);
+  if (!row_ok) return;
+  const bool good = ss < INFINITY && amax < INFINITY;  // false for NaN
+  const float top = a.format == CODES_INT8 ? 127.0f : 448.0f;
+  const float s = __fmul_rn(__fdiv_rn(fmaxf(amax, 1e-5f), top), a.clip);
+  if (t == 0) a.scale[row] = good ? s : __int_as_float(0x7fc00000);
+  const float inv = __fdiv_rn(1.0f, s);
+  uint8_t* q = static_cast<uint8_t*>(a.codes) + row * a.D;
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    if constexpr (VEC) {
+      if (at(i, 0) >= a.D) continue;
+      uint2 o = make_uint2(0u, 0u);
+      if (good) {
+        if (a.format == CODES_INT8) {
+          uint32_t c[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) c[e] = detail::code_int8(v[i][e], inv);
+          o.x = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+          o.y = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
+        } else {
+          o.x = detail::code_e4m3x2(v[i][0], v[i][1], inv) | detail::code_e4m3x2(v[i][2], v[i][3], inv) << 16;
+          o.y = detail::code_e4m3x2(v[i][4], v[i][5], inv) | detail::code_e4m3x2(v[i][6], v[i][7], inv) << 16;
+        }
+      }
+      *reinterpret_cast<uint2*>(q + at(i, 0)) = o;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (at(i, e) >= a.D) continue;
+        uint32_t c = 0;
+        if (good)
+          c = a.format == CODES_INT8 ? detail::code_int8(v[i][e], inv) : detail::code_e4m3x2(v[i][e], 0.0f, inv);
+        q[at(i, e)] = static_cast<uint8_t>(c);
+      }
+    }
+  }
+}
+
+constexpr int kRmsNormMaxD = 16384;  // a row stays in the registers of 256 threads
+
+template <typename T, bool VEC>
+inline cudaError_t launch_rms_norm_quant(const RmsNormArgs& a, cudaStream_t stream) {
+#define B200W4A4_RMS_LAUNCH(TPR, NCH)                                                             \
+  do {                                                                                             \
+    constexpr int ROWS = 256 / (TPR);                                                              \
+    const unsigned grid = static_cast<unsigned>((static_cast<long long>(a.M) + ROWS - 1) / ROWS);  \
+    rms_norm_quant_kernel<T, TPR, NCH, VEC><<<grid, 256, 0, stream>>>(a);                          \
+  } while (0)
+  const int chunks = (a.D + 7) / 8;
+  if (chunks <= 32) B200W4A4_RMS_LAUNCH(32, 1);
+  else if (chunks <= 32 * 3) B200W4A4_RMS_LAUNCH(32, 3);
+  else if (chunks <= 64 * 3) B200W4A4_RMS_LAUNCH(64, 3);
+  else if (chunks <= 128 * 3) B200W4A4_RMS_LAUNCH(128, 3);
+  else if (chunks <= 256 * 3) B200W4A4_RMS_LAUNCH(256, 3);
+  else if (chunks <= 256 * 5) B200W4A4_RMS_LAUNCH(256, 5);
+  else B200W4A4_RMS_LAUNCH(256, 8);
+#undef B200W4A4_RMS_LAUNCH
+  return cudaGetLastError();
+}
+
+}  // namespace b200w4a4

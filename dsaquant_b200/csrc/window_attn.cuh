@@ -1,0 +1,359 @@
+// Causal attention with a sliding window and a few first keys that stay visible (sinks).
+// Query i of a sequence whose cache holds `len` keys sits at position p = len - Lq + i and sees key j when
+//   j <= p  and  (j > p - window  or  j < sinks).
+//   out = sum_j softmax_j(q . k_j * scale) v_j,   lse = log sum_j exp(q . k_j * scale)
+// A query that sees nothing (p < 0) has out = 0 and lse = -inf.
+//
+// A tile is ROWS (query, head) rows of the heads that share one key head: row r is query r / G, head r % G,
+// so a cached key tile serves the whole group, for prompts and single tokens alike.  The keys that any row
+// of the tile sees are two runs of key tiles - [0, first) for the sinks and [w0, w1] for the window - and only
+// those are visited; the mask is evaluated only in tiles that some row does not see entirely.
+// Keys that no row of the tile sees are read as zeros, so whatever lies there (freed or unwritten cache
+// lines, NaN among them) has no effect.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace b200w4a4 {
+
+struct WindowAttnArgs {
+  const void *q, *k, *v;  // [B, Lq, Hq, HD], [B, Lk, Hkv, HD]
+  void* out;              // [B, Lq, Hq, HD] contiguous
+  float* lse;             // [B, Hq, Lq] or null
+  const int* kv_lens;     // [B] or null: Lk
+  long long q_b, q_t, q_h, k_b, k_t, k_h, v_b, v_t, v_h;  // pitches in elements
+  int B, Lq, Lk, Hq, Hkv, G;
+  int window, sinks;
+  float scale;
+  int splits;       // key runs a row's tiles are split into; > 1: partial results go to the workspace
+  float* part_o;    // [splits, B, Hq, Lq, HD]
+  float* part_lse;  // [splits, B, Hq, Lq], in units of log2
+};
+
+namespace attn {
+
+// What a tile of rows [r0, r1] of one sequence has to visit.
+struct Span {
+  int p0, p1;     // positions of its first and last query
+  int lo, hi;     // keys [lo, hi] cover every row's window (hi < lo: nothing)
+  int n_sink, w0, n;  // key tiles: [0, n_sink) and [w0, w0 + n - n_sink)
+};
+
+template <int BN>
+__device__ __forceinline__ Span span_of(const WindowAttnArgs& a, int b, int i0, int i1) {
+  Span s;
+  int len = a.Lk;
+  if (a.kv_lens != nullptr) len = min(max(a.kv_lens[b], 0), a.Lk);
+  s.p0 = len - a.Lq + i0;
+  s.p1 = len - a.Lq + i1;
+  s.hi = s.p1;
+  const int first = max(s.p0, 0);  // rows before position 0 see nothing
+  s.lo = max(0, first - a.window + 1);
+  if (s.hi < 0) {
+    s.n_sink = s.w0 = s.n = 0;
+    s.lo = 0;
+    return s;
+  }
+  s.w0 = s.lo / BN;
+  s.n_sink = min((min(a.sinks, s.lo) + BN - 1) / BN, s.w0);
+  s.n = s.n_sink + s.hi / BN - s.w0 + 1;
+  return s;
+}
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+// 16 bytes global -> shared; zeros when !ok (nothing is read then)
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
+  const int n = ok ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack2(float x, float y, __half) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float x, float y, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// Element offset of 16-byte chunk c of row r in a [rows][HD] tile: chunks of a row are permuted by
+// the row's low bits, so the eight rows that one ldmatrix phase touches sit in different banks.
+template <int HD>
+__device__ __forceinline__ int swz(int r, int c) {
+  return r * HD + ((c ^ (r & 7)) << 3);
+}
+
+}  // namespace attn
+
+// mma.sync form: four warps of 16 rows each, key tiles of 64 in two cp.async stages.
+constexpr int kAttnRows = 64, kAttnBN = 64;
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(128) window_attn_kernel(const WindowAttnArgs a) {
+  using namespace attn;
+  constexpr int BN = kAttnBN, KT = HD / 16;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  T* sk = reinterpret_cast<T*>(smem_raw);  // [2][BN][HD]
+  T* sv = sk + 2 * BN * HD;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int hk = blockIdx.y;
+  const int b = blockIdx.z / a.splits, split = blockIdx.z % a.splits;
+  const long long rows = static_cast<long long>(a.Lq) * a.G;
+  const long long r0 = static_cast<long long>(blockIdx.x) * kAttnRows;
+  const long long r1 = min(r0 + kAttnRows, rows) - 1;
+  const Span sp = span_of<BN>(a, b, static_cast<int>(r0 / a.G), static_cast<int>(r1 / a.G));
+  const int per = (sp.n + a.splits - 1) / a.splits;
+  const int first = min(split * per, sp.n), last = min(first + per, sp.n);
+
+  // this thread's two rows
+  int pos[2];
+  long long q_off[2];
+  bool row_ok[2];
+  int qi[2], qh[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const long long r = r0 + 16 * warp + g + 8 * i;
+    row_ok[i] = r < rows;
+    qi[i] = static_cast<int>((row_ok[i] ? r : rows - 1) / a.G);
+    qh[i] = hk * a.G + static_cast<int>((row_ok[i] ? r : rows - 1) % a.G);
+    pos[i] = sp.p0 - static_cast<int>(r0 / a.G) + qi[i];
+    q_off[i] = b * a.q_b + qi[i] * a.q_t + qh[i] * a.q_h;
+  }
+  uint32_t qf[KT][4];
+  {
+    const T* q = static_cast<const T*>(a.q);
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        qf[kt][i] = __ldg(reinterpret_cast<const uint32_t*>(q + q_off[i & 1] + 16 * kt + 2 * t + 8 * (i >> 1)));
+  }
+
+  const T* kb = static_cast<const T*>(a.k) + b * a.k_b + hk * a.k_h;
+  const T* vb = static_cast<const T*>(a.v) + b * a.v_b + hk * a.v_h;
+  auto tile_key = [&](int n) { return (n < sp.n_sink ? n : sp.w0 + n - sp.n_sink) * BN; };
+  auto load = [&](int n, int stage) {
+    const int j0 = tile_key(n);
+    constexpr int CH = HD / 8;
+#pragma unroll
+    for (int i = 0; i < BN * CH / 128; ++i) {
+      const int c = threadIdx.x + i * 128;
+      const int r = c / CH, ch = c % CH;
+      const int j = j0 + r;
+      const bool ok = j <= sp.hi && (j >= sp.lo || j < a.sinks);
+      cp16(smem_addr(sk + stage * BN * HD + swz<HD>(r, ch)), kb + (ok ? j * a.k_t + ch * 8 : 0), ok);
+      cp16(smem_addr(sv + stage * BN * HD + swz<HD>(r, ch)), vb + (ok ? j * a.v_t + ch * 8 : 0), ok);
+    }
+  };
+
+  float o[HD / 8][4];
+#pragma unroll
+  for (int i = 0; i < HD / 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+  const float sc = a.scale * kLog2e;
+
+  if (first < last) load(first, 0);
+  cp_commit();
+  for (int n = first; n < last; ++n) {
+    const int stage = (n - first) & 1;
+    if (n + 1 < last) load(n + 1, stage ^ 1);
+    cp_commit();
+    cp_wait<1>();
+    __syncthreads();
+    const T* ks = sk + stage * BN * HD;
+    const T* vs = sv + stage * BN * HD;
+    float s[BN / 8][4];
+#pragma unroll
+    for (int i = 0; i < BN / 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[i][j] = 0.0f;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+      for (int nt = 0; nt < BN / 16; ++nt) {
+        // matrices: keys 0-7 | k lo, keys 0-7 | k hi, keys 8-15 | k lo, keys 8-15 | k hi
+        uint32_t f[4];
+        ldsm4(f, smem_addr(ks + swz<HD>(16 * nt + (lane & 7) + ((lane >> 4) << 3), 2 * kt + ((lane >> 3) & 1))));
+        mma(s[2 * nt], qf[kt], f[0], f[1], T());
+        mma(s[2 * nt + 1], qf[kt], f[2], f[3], T());
+      }
+    }
+    const int j0 = tile_key(n);
+    // every row sees the whole tile when its last key is at or before the first position and its first
+    // key is inside the last position's window
+    const bool whole = j0 + BN - 1 <= sp.p0 && (j0 > sp.p1 - a.window || j0 + BN <= a.sinks);
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < BN / 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int key = j0 + 8 * i + 2 * t + (j & 1), p = pos[j >> 1];
+          if (!(key <= p && (key > p - a.window || key < a.sinks))) s[i][j] = -INFINITY;
+        }
+    }
+    float mx[2] = {m[0], m[1]};
+#pragma unroll
+    for (int i = 0; i < BN / 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mx[j >> 1] = fmaxf(mx[j >> 1], s[i][j] * sc);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+      const float base = mx[i] == -INFINITY ? 0.0f : mx[i];
+      const float f = exp2_fast(m[i] - base);
+      m[i] = mx[i];
+      l[i] *= f;
+#pragma unroll
+      for (int h = 0; h < HD / 8; ++h) {
+        o[h][2 * i] *= f;
+        o[h][2 * i + 1] *= f;
+      }
+      mx[i] = base;
+    }
+#pragma unroll
+    for (int i = 0; i < BN / 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] = exp2_fast(fmaf(s[i][j], sc, -mx[j >> 1]));
+        l[j >> 1] += s[i][j];
+      }
+#pragma unroll
+    for (int kt = 0; kt < BN / 16; ++kt) {
+      const uint32_t p[4] = {pack2(s[2 * kt][0], s[2 * kt][1], T()), pack2(s[2 * kt][2], s[2 * kt][3], T()),
+                             pack2(s[2 * kt + 1][0], s[2 * kt + 1][1], T()), pack2(s[2 * kt + 1][2], s[2 * kt + 1][3], T())};
+#pragma unroll
+      for (int ht = 0; ht < HD / 16; ++ht) {
+        // transposed: keys lo | dims 0-7, keys hi | dims 0-7, keys lo | dims 8-15, keys hi | dims 8-15
+        uint32_t f[4];
+        ldsm4t(f, smem_addr(vs + swz<HD>(16 * kt + (lane & 15), 2 * ht + (lane >> 4))));
+        mma(o[2 * ht], p, f[0], f[1], T());
+        mma(o[2 * ht + 1], p, f[2], f[3], T());
+      }
+    }
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    if (!row_ok[i]) continue;
+    const float inv = l[i] > 0.0f ? 1.0f / l[i] : (l[i] == 0.0f ? 0.0f : l[i]);
+    const float lse2 = l[i] == 0.0f ? -INFINITY : m[i] + log2f(l[i]);
+    const long long head_row = (static_cast<long long>(b) * a.Hq + qh[i]) * a.Lq + qi[i];
+    if (a.splits > 1) {
+      const long long at = static_cast<long long>(split) * a.B * a.Hq * a.Lq + head_row;
+      if (t == 0) a.part_lse[at] = lse2;
+      float2* po = reinterpret_cast<float2*>(a.part_o + at * HD) + t;
+#pragma unroll
+      for (int h = 0; h < HD / 8; ++h) po[4 * h] = make_float2(o[h][2 * i] * inv, o[h][2 * i + 1] * inv);
+    } else {
+      if (t == 0 && a.lse != nullptr) a.lse[head_row] = lse2 * kLn2;
+      T* out = static_cast<T*>(a.out) + ((static_cast<long long>(b) * a.Lq + qi[i]) * a.Hq + qh[i]) * HD + 2 * t;
+#pragma unroll
+      for (int h = 0; h < HD / 8; ++h)
+        *reinterpret_cast<uint32_t*>(out + 8 * h) = pack2(o[h][2 * i] * inv, o[h][2 * i + 1] * inv, T());
+    }
+  }
+}
+
+// Joins the partial results of the splits: one warp a (batch, head, query) row.
+template <typename T, int HD>
+__global__ void __launch_bounds__(128) window_attn_join_kernel(const WindowAttnArgs a) {
+  using namespace attn;
+  const long long rows = static_cast<long long>(a.B) * a.Hq * a.Lq;
+  const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 31;
+  float m = -INFINITY;
+  for (int s = lane; s < a.splits; s += 32) m = fmaxf(m, a.part_lse[s * rows + row]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float base = m == -INFINITY ? 0.0f : m;
+  float total = 0.0f;
+  float acc[HD / 32] = {};
+  for (int s = 0; s < a.splits; ++s) {
+    const float l = a.part_lse[s * rows + row];
+    if (l == -INFINITY) continue;  // a run without keys: its partial output is not read
+    const float w = exp2_fast(l - base);
+    total += w;
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) acc[i] = fmaf(w, a.part_o[(s * rows + row) * HD + lane + 32 * i], acc[i]);
+  }
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  const int qi = static_cast<int>(row % a.Lq);
+  const long long bh = row / a.Lq;
+  const int h = static_cast<int>(bh % a.Hq), b = static_cast<int>(bh / a.Hq);
+  if (lane == 0 && a.lse != nullptr) a.lse[row] = total == 0.0f ? -INFINITY : (base + log2f(total)) * kLn2;
+  T* out = static_cast<T*>(a.out) + ((static_cast<long long>(b) * a.Lq + qi) * a.Hq + h) * HD + lane;
+#pragma unroll
+  for (int i = 0; i < HD / 32; ++i) out[32 * i] = static_cast<T>(acc[i] * inv);
+}
+
+// Runs a tile's keys are split into: enough tiles to give every SM two CTAs, at least two key tiles a run.
+inline int window_attn_splits(int B, int Lq, int Lk, int Hkv, int G, int window, int sinks, int sm_count) {
+  const long long tiles = (static_cast<long long>(Lq) * G + kAttnRows - 1) / kAttnRows * Hkv * B;
+  if (tiles <= 0) return 1;
+  const long long reach = static_cast<long long>(window) + kAttnRows / G + 1;
+  const long long keys = Lk < reach ? Lk : (Lk < reach + sinks ? Lk : reach + sinks);
+  const long long key_tiles = (keys + kAttnBN - 1) / kAttnBN;
+  long long s = (2LL * sm_count + tiles - 1) / tiles;
+  if (s > key_tiles / 2) s = key_tiles / 2;
+  if (s > 64) s = 64;
+  return s < 1 ? 1 : static_cast<int>(s);
+}
+
+template <typename T, int HD>
+inline cudaError_t launch_window_attn(const WindowAttnArgs& a, cudaStream_t stream) {
+  constexpr int smem = 4 * kAttnBN * HD * 2;
+  cudaError_t e = cudaFuncSetAttribute(window_attn_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  const long long rows = static_cast<long long>(a.Lq) * a.G;
+  const dim3 grid(static_cast<unsigned>((rows + kAttnRows - 1) / kAttnRows), static_cast<unsigned>(a.Hkv),
+                  static_cast<unsigned>(a.B * a.splits));
+  window_attn_kernel<T, HD><<<grid, 128, smem, stream>>>(a);
+  if (a.splits > 1) {
+    const long long total = static_cast<long long>(a.B) * a.Hq * a.Lq;
+    window_attn_join_kernel<T, HD><<<static_cast<unsigned>((total + 3) / 4), 128, 0, stream>>>(a);
+  }
+  return cudaGetLastError();
+}
+
+}  // namespace b200w4a4

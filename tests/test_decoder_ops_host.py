@@ -1,0 +1,154 @@
+"""CPU-only tests of the decoder-layer operators: header and binding agree, arguments are refused before anything
+is launched, tables and packed forms are what their formulas say."""
+import math
+import re
+from pathlib import Path
+
+import pytest
+import torch
+
+ROOT = Path(__file__).resolve().parent.parent
+P = 1 << 12  # a 16-byte aligned address that no refused call may touch
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from dsaquant_b200 import _lib
+
+    return _lib.load()
+
+
+def test_header_and_binding_list_the_same_symbols(lib):
+    from dsaquant_b200 import _lib
+
+    header = (ROOT / "include" / "b200w4a4_decoder.h").read_text()
+    declared = set(re.findall(r"^(?:int|size_t) (b200w4a4_[a-z0-9_]+)\(", header, re.M))
+    assert declared == set(_lib.DECODER_SIGNATURES)
+    for name in declared:
+        assert hasattr(lib, name)
+
+
+def _rms(lib, **over):
+    a = dict(x=P, dt=1, ld=64, r=None, rld=64, w=P, wdt=1, eps=1e-6, codes=P, fmt=0, scale=P, ro=None, m=2, d=64, clip=1.0, s=None)
+    a.update(over)
+    return lib.b200w4a4_rms_norm_quant(*a.values())
+
+
+@pytest.mark.parametrize("over, code", [
+    (dict(dt=3), -1), (dict(wdt=-1), -1), (dict(fmt=2), -1), (dict(r=P), -1), (dict(ro=P), -1), (dict(clip=0.0), -1),
+    (dict(clip=float("nan")), -1), (dict(eps=-1.0), -1), (dict(m=-1), -2), (dict(d=0), -2), (dict(d=16385, ld=16385), -2),
+    (dict(x=None), -1), (dict(w=None), -1), (dict(codes=None), -1), (dict(scale=None), -1), (dict(ld=63), -2),
+    (dict(r=P, ro=P, rld=10), -2), (dict(x=P + 1), -3), (dict(scale=P + 2), -3), (dict(m=0, x=None), 0),
+])
+def test_rms_norm_quant_refusals(lib, over, code):
+    assert _rms(lib, **over) == code
+
+
+def _w4(lib, **over):
+    a = dict(x=P, dt=0, act=None, p=P, s=P, bias=None, out=P, odt=0, m=1, n=16, k=128, g=128, st=None)
+    a.update(over)
+    return lib.b200w4a4_linear_w4_group(*a.values())
+
+
+@pytest.mark.parametrize("over, code", [
+    (dict(dt=2), -1), (dict(odt=2), -1), (dict(act=P), -1), (dict(dt=3), -1), (dict(m=-1), -2), (dict(n=0), -2),
+    (dict(k=100, g=100), -2), (dict(g=48), -2), (dict(g=0), -2), (dict(k=160, g=64), -2), (dict(x=P + 8), -3),
+    (dict(p=P + 4), -3), (dict(x=None), -1), (dict(out=None), -1), (dict(m=65535 * 8 + 1), -2), (dict(m=0, x=None), 0),
+])
+def test_linear_w4_group_refusals(lib, over, code):
+    assert _w4(lib, **over) == code
+
+
+@pytest.mark.parametrize("args, code", [
+    ((None, 0, P, P, 4, 64, 32, None), -1), ((P, 5, P, P, 4, 64, 32, None), -1), ((P, 0, P, P, 0, 64, 32, None), -2),
+    ((P, 0, P, P, 4, 80, 32, None), -2), ((P, 0, P, P, 4, 64, 16, None), -2), ((P + 1, 0, P, P, 4, 64, 32, None), -3),
+])
+def test_quantize_weight_grouped_refusals(lib, args, code):
+    assert lib.b200w4a4_quantize_weight_grouped(*args) == code
+
+
+def _rot(lib, **over):
+    a = dict(q=P, qt=256, qh=64, qo=P, qot=256, qoh=64, hq=4, k=P, kt=64, kh=64, ko=P, kot=64, koh=64, hk=1, dt=1, cs=P, mp=10,
+             pos=P, p64=1, t=3, hd=64, rd=64, il=0, inv=0, st=None)
+    a.update(over)
+    return lib.b200w4a4_rotary(*a.values())
+
+
+@pytest.mark.parametrize("over, code", [
+    (dict(dt=3), -1), (dict(p64=2), -1), (dict(il=2), -1), (dict(inv=-1), -1), (dict(t=-1), -2), (dict(hq=0), -2),
+    (dict(hk=-1), -2), (dict(mp=0), -2), (dict(hd=513), -2), (dict(rd=66), -2), (dict(rd=63), -2), (dict(rd=0), -2),
+    (dict(q=None), -1), (dict(k=None), -1), (dict(cs=None), -1), (dict(pos=None), -1), (dict(pos=P + 4), -3),
+    (dict(cs=P + 4), -3), (dict(ko=P + 1), -3), (dict(t=0, q=None), 0),
+])
+def test_rotary_refusals(lib, over, code):
+    assert _rot(lib, **over) == code
+
+
+def _attn(lib, **over):
+    a = dict(q=P, qb=256, qt=128, qh=64, k=P, kb=256, kt=64, kh=64, v=P, vb=256, vt=64, vh=64, lens=None, out=P, lse=None, dt=1,
+             b=1, lq=1, lk=4, hq=2, hk=1, hd=64, w=4, s=0, scale=0.125, ws=None, wb=0, st=None)
+    a.update(over)
+    return lib.b200w4a4_window_attention(*a.values())
+
+
+@pytest.mark.parametrize("over, code", [
+    (dict(dt=2), -1), (dict(hd=96), -2), (dict(hq=3, hk=2), -2), (dict(hq=65, hk=1), -2), (dict(hk=0), -2), (dict(b=-1), -2),
+    (dict(b=65536), -2), (dict(lq=-1), -2), (dict(lk=-1), -2), (dict(w=0), -1), (dict(s=-1), -1), (dict(scale=0.0), -1),
+    (dict(scale=-1.0), -1), (dict(scale=float("nan")), -1), (dict(q=None), -1), (dict(k=None), -1), (dict(out=None), -1),
+    (dict(q=P + 8), -3), (dict(kt=68), -3), (dict(ws=P + 4), -3), (dict(lens=P + 2), -3), (dict(b=0, q=None), 0),
+    (dict(lq=0, q=None), 0), (dict(lq=1 << 30, hq=64, hk=1), -2),
+])
+def test_window_attention_refusals(lib, over, code):
+    assert _attn(lib, **over) == code
+
+
+def test_python_wrappers_refuse_cpu_tensors_and_bad_tables():
+    from dsaquant_b200.kernels.rms_norm import rms_norm_quant
+    from dsaquant_b200.kernels.w4_group import linear_w4_group, quantize_weight_grouped
+    from dsaquant_b200.rotary import apply_rotary, rotary_table
+    from dsaquant_b200.window_attention import window_attention
+
+    x = torch.zeros(2, 64, dtype=torch.float16)
+    with pytest.raises(RuntimeError):
+        rms_norm_quant(x, torch.ones(64))
+    with pytest.raises(RuntimeError):
+        quantize_weight_grouped(x, 32)
+    with pytest.raises(RuntimeError):
+        linear_w4_group(x, torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.float16))
+    with pytest.raises(RuntimeError):
+        apply_rotary(x.view(2, 1, 64), None, rotary_table(4, 64), torch.arange(2))
+    with pytest.raises(RuntimeError):
+        window_attention(x.view(1, 2, 1, 64), x.view(1, 2, 1, 64), x.view(1, 2, 1, 64), 4)
+    for bad in (dict(max_positions=0, rotary_dim=64), dict(max_positions=4, rotary_dim=63), dict(max_positions=4, rotary_dim=64, scaling="x"),
+                dict(max_positions=4, rotary_dim=64, factor=0.5), dict(max_positions=4, rotary_dim=2, scaling="ntk")):
+        with pytest.raises(ValueError):
+            rotary_table(**bad)
+
+
+def test_rotary_tables_follow_their_formulas():
+    from dsaquant_b200.rotary import rotary_table
+
+    rd, far = 64, 70000
+    plain = rotary_table(far, rd, 10000.0)
+    assert plain.shape == (far, rd // 2, 2) and plain.dtype == torch.float32
+    for p, i in ((0, 0), (1, 0), (69999, 0), (69999, 31), (12345, 7)):
+        angle = p * 10000.0 ** (-2 * i / rd)
+        # one rounding to fp32 (half an eps) of a 64-bit cosine whose angle is exact to 2^-53 of itself
+        for got, want in zip(plain[p, i].tolist(), (math.cos(angle), math.sin(angle))):
+            assert abs(got - want) <= 2.0 ** -24 * max(abs(want), 1e-30) + far * 2.0 ** -50
+    linear = rotary_table(1000, rd, scaling="linear", factor=4.0)
+    assert torch.equal(linear[::4], plain[:250])
+    ntk = rotary_table(1000, rd, scaling="ntk", factor=4.0)
+    assert torch.equal(ntk[:, 0], plain[:1000, 0])                       # the fastest pair stays
+    slow = 10000.0 ** (-2 * 31 / rd) / 4.0                               # the slowest is stretched by the factor
+    assert abs(ntk[999, 31, 1].item() - math.sin(999 * slow)) < 1e-6
+    yarn = rotary_table(1000, rd, scaling="yarn", factor=4.0, trained_positions=4096)
+    amp = 0.1 * math.log(4.0) + 1
+    assert torch.allclose(yarn[:, 0], plain[:1000, 0] * amp, rtol=3e-7, atol=1e-7)
+    assert abs(yarn[999, 31, 1].item() - amp * math.sin(999 * slow)) < 1e-6
+    assert abs(rotary_table(4, rd, scaling="yarn", factor=1.0) - rotary_table(4, rd)).max().item() == 0.0
+
+
+def test_workspace_query_of_bad_or_empty_shapes_is_zero(lib):
+    assert lib.b200w4a4_window_attention_workspace_bytes(0, 1, 4, 2, 1, 64, 4, 0) == 0
+    assert lib.b200w4a4_window_attention_workspace_bytes(1, 1, 4, 3, 2, 64, 4, 0) == 0
