@@ -117,6 +117,12 @@ int device_state(DeviceState** out) {
   return st.err;
 }
 
+unsigned next_launch_id(DeviceState& st) {
+  unsigned id = st.launch_seq.fetch_add(1, std::memory_order_relaxed) + 1;
+  if (id == 0) id = st.launch_seq.fetch_add(1, std::memory_order_relaxed) + 1;  // 0 means "no launch"
+  return id;
+}
+
 int current_cta_group() {
   int g = g_cta_group.load(std::memory_order_relaxed);
   if (g == 0) {
@@ -272,9 +278,7 @@ int launch_gemm_staged(DeviceState& st, const void* qact, const float* act_scale
   p.n_tiles = (N + C::BN - 1) / C::BN;
   p.status = st.status_ptr;
   p.abort_word = st.abort_ptr;
-  unsigned id = st.launch_seq.fetch_add(1, std::memory_order_relaxed) + 1;
-  if (id == 0) id = st.launch_seq.fetch_add(1, std::memory_order_relaxed) + 1;  // 0 means "no launch"
-  p.launch_id = id;
+  p.launch_id = next_launch_id(st);
   p.residual = epi.residual;
   p.gate = epi.gate;
   p.gate_row_stride = epi.gate_row_stride;
@@ -346,13 +350,20 @@ int noalloc_scratch(uint8_t** base) {
 
 }  // namespace
 
-int b200w4a4::current_device(int* sm_count, int** status) {
+int b200w4a4::current_device(DeviceInfo* info) {
   DeviceState* st = nullptr;
   const int rc = device_state(&st);
-  if (rc == B200W4A4_OK && sm_count != nullptr) *sm_count = st->sm_count;
-  if (rc == B200W4A4_OK && status != nullptr) *status = st->status_ptr;
+  if (rc == B200W4A4_OK && info != nullptr) *info = DeviceInfo{st->sm_count, st->status_ptr, st->abort_ptr};
   return rc;
 }
+
+unsigned b200w4a4::new_launch_id() {
+  DeviceState* st = nullptr;
+  if (device_state(&st) != B200W4A4_OK) return 1;
+  return next_launch_id(*st);
+}
+
+void* b200w4a4::tensor_map_encoder() { return reinterpret_cast<void*>(get_encode()); }
 
 extern "C" {
 

@@ -18,7 +18,7 @@ ROOT = CSRC.parent.parent
 LIB_NAME = "libb200w4a4.so"
 SOURCES = ["b200w4a4_api.cu", "decoder_api.cu"]
 HEADERS = ["gemm_w4a4.cuh", "quant_act.cuh", "weight_pack.cuh", "ptx.cuh", "attn_glue.cuh", "device_state.cuh",
-           "rms_norm.cuh", "rotary.cuh", "w4_group.cuh", "window_attn.cuh"]
+           "rms_norm.cuh", "rotary.cuh", "w4_group.cuh", "window_attn.cuh", "window_attn_tc.cuh"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",

@@ -11,6 +11,7 @@
 #include "rotary.cuh"
 #include "w4_group.cuh"
 #include "window_attn.cuh"
+#include "window_attn_tc.cuh"
 
 namespace {
 
@@ -24,13 +25,14 @@ int launched(cudaError_t e) { return e == cudaSuccess ? B200W4A4_OK : B200W4A4_E
 int attention_splits(int B, int Lq, int Lk, int q_heads, int k_heads, int window, int sinks, int sm_count) {
   if (window > Lk) window = Lk;
   if (sinks > Lk) sinks = Lk;
+  if (Lq >= kAttnTcMinQueries) return 1;
   int s = window_attn_splits(B, Lq, Lk, k_heads, q_heads / k_heads, window, sinks, sm_count);
   if (static_cast<long long>(B) * s > 65535) s = 65535 / B;
   return s < 1 ? 1 : s;
 }
 
 bool attention_shape_ok(int B, int Lq, int Lk, int q_heads, int k_heads, int head_dim) {
-  return B >= 0 && B <= 65535 && Lq >= 0 && Lk >= 0 && q_heads >= 1 && k_heads >= 1 && k_heads <= 65535 &&
+  return B >= 0 && B <= 65535 && Lq >= 0 && Lk >= 0 && q_heads >= 1 && k_heads >= 1 && q_heads <= 65535 &&
          q_heads % k_heads == 0 && q_heads / k_heads <= 64 && (head_dim == 64 || head_dim == 128) &&
          static_cast<long long>(Lq) * (q_heads / k_heads) <= 0x7fffffffLL - kAttnRows && Lk <= 0x7fffffff - 1024;
 }
@@ -55,7 +57,7 @@ int b200w4a4_rms_norm_quant(const void* x, int x_dtype, long long x_ld, const vo
   if (!aligned(x, es) || !aligned(residual, es) || !aligned(residual_out, es) || !aligned(weight, size_of(w_dtype)) ||
       !aligned(scale, 4))
     return B200W4A4_EALIGN;
-  const int rc = current_device(nullptr, nullptr);
+  const int rc = current_device(nullptr);
   if (rc != B200W4A4_OK) return rc;
   RmsNormArgs a;
   a.x = x;
@@ -90,7 +92,7 @@ int b200w4a4_quantize_weight_grouped(const void* w, int w_dtype, void* packed, v
   if (w == nullptr || packed == nullptr || scale == nullptr || !float_dtype(w_dtype)) return B200W4A4_EINVAL;
   if (N < 1 || K < 32 || group < 32 || group % 32 != 0 || K % group != 0) return B200W4A4_ESHAPE;
   if (!aligned(w, size_of(w_dtype)) || !aligned(scale, 2)) return B200W4A4_EALIGN;
-  const int rc = current_device(nullptr, nullptr);
+  const int rc = current_device(nullptr);
   if (rc != B200W4A4_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint8_t* p = static_cast<uint8_t*>(packed);
@@ -115,7 +117,7 @@ int b200w4a4_linear_w4_group(const void* x, int x_dtype, const float* act_scale,
   if (!aligned(x, 16) || !aligned(packed, 16) || !aligned(scale, 2) || !aligned(out, 2) || !aligned(bias, 2) ||
       !aligned(act_scale, 4))
     return B200W4A4_EALIGN;
-  const int rc = current_device(nullptr, nullptr);
+  const int rc = current_device(nullptr);
   if (rc != B200W4A4_OK) return rc;
   W4GroupArgs a;
   a.x = x;
@@ -161,7 +163,7 @@ int b200w4a4_rotary(const void* q, long long q_tok, long long q_head, void* q_ou
   if (!aligned(q, es) || !aligned(q_out, es) || !aligned(cos_sin, 8) || !aligned(positions, positions_int64 ? 8 : 4))
     return B200W4A4_EALIGN;
   if (k_heads > 0 && (!aligned(k, es) || !aligned(k_out, es))) return B200W4A4_EALIGN;
-  const int rc = current_device(nullptr, nullptr);
+  const int rc = current_device(nullptr);
   if (rc != B200W4A4_OK) return rc;
   RotaryArgs a;
   a.in[0] = q; a.in_tok[0] = q_tok; a.in_head[0] = q_head;
@@ -194,9 +196,9 @@ int b200w4a4_rotary(const void* q, long long q_tok, long long q_head, void* q_ou
 size_t b200w4a4_window_attention_workspace_bytes(int B, int Lq, int Lk, int q_heads, int k_heads,
                                                  int head_dim, int window, int sinks) {
   if (!attention_shape_ok(B, Lq, Lk, q_heads, k_heads, head_dim) || window < 1 || sinks < 0 || B == 0 || Lq == 0) return 0;
-  int sm_count = 0;
-  if (current_device(&sm_count, nullptr) != B200W4A4_OK) return 0;
-  const int splits = attention_splits(B, Lq, Lk, q_heads, k_heads, window, sinks, sm_count);
+  DeviceInfo dev;
+  if (current_device(&dev) != B200W4A4_OK) return 0;
+  const int splits = attention_splits(B, Lq, Lk, q_heads, k_heads, window, sinks, dev.sm_count);
   if (splits == 1) return 0;
   return static_cast<size_t>(splits) * B * q_heads * Lq * (head_dim + 1) * sizeof(float);
 }
@@ -218,8 +220,8 @@ int b200w4a4_window_attention(const void* q, long long q_b, long long q_tok, lon
   const long long pitches[9] = {q_b, q_tok, q_head, k_b, k_tok, k_head, v_b, v_tok, v_head};
   for (long long p : pitches)
     if (p % 8 != 0) return B200W4A4_EALIGN;
-  int sm_count = 0;
-  const int rc = current_device(&sm_count, nullptr);
+  DeviceInfo dev;
+  const int rc = current_device(&dev);
   if (rc != B200W4A4_OK) return rc;
   WindowAttnArgs a;
   a.q = q; a.k = k; a.v = v;
@@ -234,7 +236,7 @@ int b200w4a4_window_attention(const void* q, long long q_b, long long q_tok, lon
   a.window = window > Lk ? (Lk > 0 ? Lk : 1) : window;
   a.sinks = sinks > Lk ? Lk : sinks;
   a.scale = scale;
-  a.splits = attention_splits(B, Lq, Lk, q_heads, k_heads, window, sinks, sm_count);
+  a.splits = attention_splits(B, Lq, Lk, q_heads, k_heads, window, sinks, dev.sm_count);
   a.part_o = a.part_lse = nullptr;
   if (a.splits > 1) {
     const size_t rows = static_cast<size_t>(a.splits) * B * q_heads * Lq;
@@ -244,6 +246,11 @@ int b200w4a4_window_attention(const void* q, long long q_b, long long q_tok, lon
     a.part_lse = a.part_o + rows * head_dim;
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (a.Lq >= kAttnTcMinQueries && a.Lk > 0) {
+    if (dtype == B200W4A4_F16)
+      return head_dim == 64 ? launch_window_attn_tc<__half, 64>(a, dev, s) : launch_window_attn_tc<__half, 128>(a, dev, s);
+    return head_dim == 64 ? launch_window_attn_tc<__nv_bfloat16, 64>(a, dev, s) : launch_window_attn_tc<__nv_bfloat16, 128>(a, dev, s);
+  }
   if (dtype == B200W4A4_F16)
     return launched(head_dim == 64 ? launch_window_attn<__half, 64>(a, s) : launch_window_attn<__half, 128>(a, s));
   return launched(head_dim == 64 ? launch_window_attn<__nv_bfloat16, 64>(a, s) : launch_window_attn<__nv_bfloat16, 128>(a, s));
