@@ -110,14 +110,15 @@ int b200w4a4_linear_w4_group(const void* x, int x_dtype, const float* act_scale,
   if (x_dtype != B200W4A4_F16 && x_dtype != B200W4A4_BF16 && x_dtype != B200W4A4_X_INT8) return B200W4A4_EINVAL;
   if (out_dtype != B200W4A4_F16 && out_dtype != B200W4A4_BF16) return B200W4A4_EINVAL;
   if (M < 0 || N < 1 || K < 32 || group < 32 || group % 32 != 0 || K % group != 0) return B200W4A4_ESHAPE;
-  if (M > 65535 * 8) return B200W4A4_ESHAPE;
+  if (M > 65535 * 8 || K > (1 << 20)) return B200W4A4_ESHAPE;
   if (M == 0) return B200W4A4_OK;
   if (x == nullptr || packed == nullptr || scale == nullptr || out == nullptr) return B200W4A4_EINVAL;
   if ((x_dtype == B200W4A4_X_INT8) != (act_scale != nullptr)) return B200W4A4_EINVAL;
   if (!aligned(x, 16) || !aligned(packed, 16) || !aligned(scale, 2) || !aligned(out, 2) || !aligned(bias, 2) ||
       !aligned(act_scale, 4))
     return B200W4A4_EALIGN;
-  const int rc = current_device(nullptr);
+  DeviceInfo dev;
+  const int rc = current_device(&dev);
   if (rc != B200W4A4_OK) return rc;
   W4GroupArgs a;
   a.x = x;
@@ -135,9 +136,9 @@ int b200w4a4_linear_w4_group(const void* x, int x_dtype, const float* act_scale,
   // the widest run of codes that surely shares a scale
   const int gb = group % 128 == 0 ? 128 : group % 64 == 0 ? 64 : 32;
 #define B200W4A4_W4G_DISPATCH(X)                                       \
-  launched(gb == 128  ? launch_w4_group<X, 128>(a, s)                  \
-           : gb == 64 ? launch_w4_group<X, 64>(a, s)                   \
-                      : launch_w4_group<X, 32>(a, s))
+  launched(gb == 128  ? launch_w4_group<X, 128>(a, dev.sm_count, s)                  \
+           : gb == 64 ? launch_w4_group<X, 64>(a, dev.sm_count, s)                   \
+                      : launch_w4_group<X, 32>(a, dev.sm_count, s))
   if (x_dtype == B200W4A4_F16) return B200W4A4_W4G_DISPATCH(__half);
   if (x_dtype == B200W4A4_BF16) return B200W4A4_W4G_DISPATCH(__nv_bfloat16);
   return B200W4A4_W4G_DISPATCH(int8_t);

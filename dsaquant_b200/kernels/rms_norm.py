@@ -9,7 +9,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _lib
-from .vdm_w4a4 import _DTYPE_CODE, _DeviceGuard, _load_ext, _require_cuda, _stream_ptr
+from .vdm_w4a4 import _DTYPE_CODE, _DeviceGuard, _empty, _load_ext, _require_cuda, _stream_ptr
 
 _FORMATS = {torch.int8: 0, torch.float8_e4m3fn: 1}
 MAX_WIDTH = 16384
@@ -17,7 +17,7 @@ MAX_WIDTH = 16384
 
 def _rows(x: torch.Tensor, d: int) -> torch.Tensor:
     """x as [rows, d] with unit column stride; a view wherever the rows have one pitch."""
-    x2 = x.reshape(-1, d)
+    x2 = x if x.dim() == 2 else x.reshape(-1, d)
     if (d > 1 and x2.stride(1) != 1) or (x2.shape[0] > 1 and x2.stride(0) < d):
         x2 = x2.contiguous()
     return x2
@@ -60,12 +60,12 @@ def rms_norm_quant(
         if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != dev:
             raise ValueError("residual must have x's shape, dtype and device")
         r2 = _rows(residual, d)
-        stream_out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        stream_out = _empty(x.shape, x.dtype, dev)
     x2 = _rows(x, d)
     m = x2.shape[0]
     w = weight if weight.is_contiguous() else weight.contiguous()
-    codes = torch.empty(x.shape, dtype=out_dtype, device=dev)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    codes = _empty(x.shape, out_dtype, dev)
+    scale = _empty(x.shape[:-1], torch.float32, dev)
     if m > 0:
         with _DeviceGuard(dev):
             rc = lib.b200w4a4_rms_norm_quant(

@@ -12,7 +12,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _lib
-from .vdm_w4a4 import _DTYPE_CODE, _DeviceGuard, _load_ext, _require_cuda, _stream_ptr
+from .vdm_w4a4 import _DTYPE_CODE, _DeviceGuard, _empty, _load_ext, _require_cuda, _stream_ptr
 
 _X_CODE = {torch.float16: 0, torch.bfloat16: 1, torch.int8: 3}
 _OUT_CODE = {torch.float16: 0, torch.bfloat16: 1}
@@ -71,7 +71,7 @@ def linear_w4_group(
         out_dtype = torch.float16 if x.dtype == torch.int8 else x.dtype
     if out_dtype not in _OUT_CODE:
         raise ValueError("out_dtype must be float16 or bfloat16")
-    x2 = x.reshape(-1, k)
+    x2 = x if x.dim() == 2 else x.reshape(-1, k)
     if not x2.is_contiguous() or x2.data_ptr() % 16:
         x2 = x2.clone(memory_format=torch.contiguous_format)
     m = x2.shape[0]
@@ -88,7 +88,7 @@ def linear_w4_group(
             raise ValueError("bias must have N elements")
         if bias.dtype != out_dtype or not bias.is_contiguous():
             bias = bias.detach().to(out_dtype).contiguous()
-    out = torch.empty(x.shape[:-1] + (n,), dtype=out_dtype, device=dev)
+    out = _empty((*x.shape[:-1], n), out_dtype, dev)
     if m > 0:
         with _DeviceGuard(dev):
             rc = lib.b200w4a4_linear_w4_group(

@@ -11,7 +11,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .kernels.vdm_w4a4 import _DTYPE_CODE, _DeviceGuard, _load_ext, _require_cuda, _stream_ptr
+from .kernels.vdm_w4a4 import _DTYPE_CODE, _DeviceGuard, _empty, _load_ext, _require_cuda, _stream_ptr
 
 SCALINGS = ("none", "linear", "ntk", "yarn")
 
@@ -110,18 +110,17 @@ def apply_rotary(
     if inplace:
         q_out, k_out = q, k
     else:
-        q_out = torch.empty((t, hq, hd), dtype=q.dtype, device=dev)
-        k_out = torch.empty((t, hk, hd), dtype=q.dtype, device=dev) if k is not None else None
+        q_out = _empty((t, hq, hd), q.dtype, dev)
+        k_out = _empty((t, hk, hd), q.dtype, dev) if k is not None else None
     if t > 0:
         pos = positions if positions.is_contiguous() else positions.contiguous()
+        qs, qos = q.stride(), q_out.stride()
+        ks, kos = (k.stride(), k_out.stride()) if k is not None else ((0, 0), (0, 0))
         with _DeviceGuard(dev):
             rc = lib.b200w4a4_rotary(
-                q.data_ptr(), q.stride(0), q.stride(1), q_out.data_ptr(), q_out.stride(0), q_out.stride(1), hq,
-                k.data_ptr() if k is not None else None, k.stride(0) if k is not None else 0,
-                k.stride(1) if k is not None else 0, k_out.data_ptr() if k is not None else None,
-                k_out.stride(0) if k is not None else 0, k_out.stride(1) if k is not None else 0, hk,
-                _DTYPE_CODE[q.dtype], cos_sin.data_ptr(), cos_sin.shape[0], pos.data_ptr(),
-                1 if pos.dtype == torch.int64 else 0, t, hd, rd, 1 if interleaved else 0, 1 if inverse else 0,
-                _stream_ptr(dev))
+                q.data_ptr(), qs[0], qs[1], q_out.data_ptr(), qos[0], qos[1], hq, k.data_ptr() if k is not None else None,
+                ks[0], ks[1], k_out.data_ptr() if k is not None else None, kos[0], kos[1], hk, _DTYPE_CODE[q.dtype],
+                cos_sin.data_ptr(), cos_sin.shape[0], pos.data_ptr(), 1 if pos.dtype == torch.int64 else 0, t, hd, rd,
+                1 if interleaved else 0, 1 if inverse else 0, _stream_ptr(dev))
         _lib.check(rc, "rotary")
     return q_out, k_out

@@ -7,16 +7,24 @@ from typing import Optional, Tuple, Union
 import torch
 
 from . import _lib
-from .kernels.vdm_w4a4 import _DeviceGuard, _load_ext, _require_cuda, _stream_ptr
+from .kernels.vdm_w4a4 import _DeviceGuard, _empty, _load_ext, _require_cuda, _stream_ptr
 
 _CODE = {torch.float16: 0, torch.bfloat16: 1}
 
 
-def _readable(x: torch.Tensor) -> torch.Tensor:
-    """x itself when the kernel can read it in place (unit stride in the head, 16-byte steps), else a copy."""
-    if x.stride(3) == 1 and x.data_ptr() % 16 == 0 and not (x.stride(0) | x.stride(1) | x.stride(2)) & 7:
-        return x
-    return x.clone(memory_format=torch.contiguous_format)
+def _readable(x: torch.Tensor) -> Tuple[torch.Tensor, Tuple[int, ...]]:
+    """x itself and its pitches when the kernel can read it in place (unit stride in the head, 16-byte steps), else a
+    copy's.  The pitch of a dimension of one is 0: it is never used."""
+    if x.data_ptr() % 16 or x.stride(3) != 1:
+        x = x.clone(memory_format=torch.contiguous_format)
+    s0, s1, s2, _ = x.stride()
+    if (s0 | s1 | s2) & 7:
+        n0, n1, n2, _ = x.shape
+        s0, s1, s2 = s0 if n0 > 1 else 0, s1 if n1 > 1 else 0, s2 if n2 > 1 else 0
+        if (s0 | s1 | s2) & 7:
+            x = x.clone(memory_format=torch.contiguous_format)
+            s0, s1, s2, _ = x.stride()
+    return x, (s0, s1, s2)
 
 
 def window_attention(
@@ -64,18 +72,17 @@ def window_attention(
         if kv_lens.dtype != torch.int32 or kv_lens.dim() != 1 or kv_lens.shape[0] != b or kv_lens.device != dev:
             raise ValueError("kv_lens must be int32 [B] on q's device")
         kv_lens = kv_lens.contiguous()
-    out = torch.empty((b, lq, hq, hd), dtype=q.dtype, device=dev)
-    lse = torch.empty((b, hq, lq), dtype=torch.float32, device=dev) if return_lse else None
+    out = _empty((b, lq, hq, hd), q.dtype, dev)
+    lse = _empty((b, hq, lq), torch.float32, dev) if return_lse else None
     if out.numel() > 0:
-        q, k, v = _readable(q), _readable(k), _readable(v)
+        (q, qs), (k, ks), (v, vs) = _readable(q), _readable(k), _readable(v)
         window, sinks = min(window, max(lk, 1)), min(sinks, lk)
         with _DeviceGuard(dev):
             need = lib.b200w4a4_window_attention_workspace_bytes(b, lq, lk, hq, hk, hd, window, sinks)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+            ws = _empty((need,), torch.uint8, dev) if need else None
             rc = lib.b200w4a4_window_attention(
-                q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), k.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
-                v.data_ptr(), v.stride(0), v.stride(1), v.stride(2), kv_lens.data_ptr() if kv_lens is not None else None,
+                q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs, kv_lens.data_ptr() if kv_lens is not None else None,
                 out.data_ptr(), lse.data_ptr() if lse is not None else None, _CODE[q.dtype], b, lq, lk, hq, hk, hd, window,
-                sinks, float(scale), ws.data_ptr() if ws is not None else None, need, _stream_ptr(dev))
+                sinks, scale, ws.data_ptr() if ws is not None else None, need, _stream_ptr(dev))
         _lib.check(rc, "window_attention")
     return (out, lse) if return_lse else out

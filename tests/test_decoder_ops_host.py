@@ -102,7 +102,10 @@ def test_window_attention_refusals(lib, over, code):
     assert _attn(lib, **over) == code
 
 
-def test_python_wrappers_refuse_cpu_tensors_and_bad_tables():
+def test_python_wrappers_refuse_cpu_tensors_and_bad_tables(monkeypatch):
+    from dsaquant_b200.kernels import vdm_w4a4
+
+    monkeypatch.setattr(vdm_w4a4, "_EXT", None)  # the loaded library is not left behind for tests of its loading
     from dsaquant_b200.kernels.rms_norm import rms_norm_quant
     from dsaquant_b200.kernels.w4_group import linear_w4_group, quantize_weight_grouped
     from dsaquant_b200.rotary import apply_rotary, rotary_table
