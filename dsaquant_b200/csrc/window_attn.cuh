@@ -294,6 +294,203 @@ __global__ void __launch_bounds__(128) window_attn_kernel(const WindowAttnArgs a
   }
 }
 
+// Single tokens: at most 16 rows a tile.  What bounds it is reading the keys and values once, so a CTA's four warps
+// each take 16 keys of every 64-key tile through a ring of their own (cp.async, kAttnDecodeStages deep, no barrier
+// between the warps), keep their own maximum, sum and output, and meet at the end in shared memory.
+constexpr int kAttnDecodeRows = 16, kAttnDecodeStages = 3;
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(128) window_attn_decode_kernel(const WindowAttnArgs a) {
+  using namespace attn;
+  constexpr int BN = kAttnBN, WN = 16, KT = HD / 16, CH = HD / 8, D = kAttnDecodeStages;
+  constexpr int TILE = WN * HD;  // values of a warp's K (or V) tile
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int hk = blockIdx.y;
+  const int b = blockIdx.z / a.splits, split = blockIdx.z % a.splits;
+  const int rows = a.Lq * a.G;
+  const int r0 = blockIdx.x * kAttnDecodeRows;
+  const int r1 = min(r0 + kAttnDecodeRows, rows) - 1;
+  const Span sp = span_of<BN>(a, b, r0 / a.G, r1 / a.G);
+  const int per = (sp.n + a.splits - 1) / a.splits;
+  const int first = min(split * per, sp.n), last = min(first + per, sp.n);
+
+  T* ring = reinterpret_cast<T*>(smem_raw) + warp * (D * 2 * TILE);
+  const T* kb = static_cast<const T*>(a.k) + b * a.k_b + hk * a.k_h;
+  const T* vb = static_cast<const T*>(a.v) + b * a.v_b + hk * a.v_h;
+  auto tile_key = [&](int n) { return (n < sp.n_sink ? n : sp.w0 + n - sp.n_sink) * BN + warp * WN; };
+  auto load = [&](int n, int stage) {
+    const int j0 = tile_key(n);
+    T* sk = ring + stage * (2 * TILE);
+#pragma unroll
+    for (int i = 0; i < WN * CH / 32; ++i) {
+      const int r = lane / CH + i * (32 / CH), ch = lane % CH;
+      const long long j = j0 + r;
+      const bool ok = j <= sp.hi && (j >= sp.lo || j < a.sinks);
+      cp16(smem_addr(sk + swz<HD>(r, ch)), kb + (ok ? j * a.k_t + ch * 8 : 0), ok);
+      cp16(smem_addr(sk + TILE + swz<HD>(r, ch)), vb + (ok ? j * a.v_t + ch * 8 : 0), ok);
+    }
+  };
+#pragma unroll
+  for (int d = 0; d < D - 1; ++d) {
+    if (first + d < last) load(first + d, d);
+    cp_commit();
+  }
+
+  int pos[2];
+  uint32_t qf[KT][4];
+  {
+    const T* q = static_cast<const T*>(a.q);
+    long long off[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = min(r0 + g + 8 * i, rows - 1);  // rows behind the last one repeat it and are not stored
+      pos[i] = sp.p0 - r0 / a.G + r / a.G;
+      off[i] = b * a.q_b + (r / a.G) * a.q_t + (hk * a.G + r % a.G) * a.q_h;
+    }
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        qf[kt][i] = __ldg(reinterpret_cast<const uint32_t*>(q + off[i & 1] + 16 * kt + 2 * t + 8 * (i >> 1)));
+  }
+
+  float o[HD / 8][4];
+#pragma unroll
+  for (int i = 0; i < HD / 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+  const float sc = a.scale * kLog2e;
+
+  int stage = 0;
+  for (int n = first; n < last; ++n) {
+    cp_wait<D - 2>();
+    __syncwarp();  // the warp's copies have landed, and it is done with the stage that is filled next
+    if (n + D - 1 < last) load(n + D - 1, stage == 0 ? D - 1 : stage - 1);
+    cp_commit();
+    const T* ks = ring + stage * (2 * TILE);
+    const T* vs = ks + TILE;
+    stage = stage == D - 1 ? 0 : stage + 1;
+    const int j0 = tile_key(n);
+    if (j0 > sp.p1) continue;  // this warp's share of the last tile is behind every row
+    float s[2][4] = {};
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      uint32_t f[4];
+      ldsm4(f, smem_addr(ks + swz<HD>((lane & 7) + ((lane >> 4) << 3), 2 * kt + ((lane >> 3) & 1))));
+      mma(s[0], qf[kt], f[0], f[1], T());
+      mma(s[1], qf[kt], f[2], f[3], T());
+    }
+    const bool whole = j0 + WN - 1 <= sp.p0 && (j0 > sp.p1 - a.window || j0 + WN <= a.sinks);
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int key = j0 + 8 * i + 2 * t + (j & 1), p = pos[j >> 1];
+          if (!(key <= p && (key > p - a.window || key < a.sinks))) s[i][j] = -INFINITY;
+        }
+    }
+    float mx[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mx[i] = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1])) * sc;
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+    }
+    // the maximum moves only when a weight would pass 2^8: sums and outputs are fp32, weights 16 bits up to 256
+    const bool move0 = mx[0] > m[0] + 8.0f, move1 = mx[1] > m[1] + 8.0f;
+    if (__any_sync(0xffffffffu, move0 || move1)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float next = (i ? move1 : move0) ? mx[i] : m[i];
+        const float f = next == m[i] ? 1.0f : exp2_fast(m[i] - next);
+        m[i] = next;
+        l[i] *= f;
+#pragma unroll
+        for (int h = 0; h < HD / 8; ++h) {
+          o[h][2 * i] *= f;
+          o[h][2 * i + 1] *= f;
+        }
+      }
+    }
+    const float neg[2] = {m[0] == -INFINITY ? 0.0f : -m[0], m[1] == -INFINITY ? 0.0f : -m[1]};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] = exp2_fast(fmaf(s[i][j], sc, neg[j >> 1]));
+        l[j >> 1] += s[i][j];
+      }
+    const uint32_t p[4] = {pack2(s[0][0], s[0][1], T()), pack2(s[0][2], s[0][3], T()), pack2(s[1][0], s[1][1], T()),
+                           pack2(s[1][2], s[1][3], T())};
+#pragma unroll
+    for (int ht = 0; ht < HD / 16; ++ht) {
+      uint32_t f[4];
+      ldsm4t(f, smem_addr(vs + swz<HD>(lane & 15, 2 * ht + (lane >> 4))));
+      mma(o[2 * ht], p, f[0], f[1], T());
+      mma(o[2 * ht + 1], p, f[2], f[3], T());
+    }
+  }
+
+  // the four warps' results: [warp][row][HD] outputs, then maxima and sums
+  constexpr int OP = HD + 8;  // row pitch: the rows of a store land in different banks
+  float* po = reinterpret_cast<float*>(smem_raw);
+  float* pm = po + 4 * kAttnDecodeRows * OP;
+  float* pl = pm + 4 * kAttnDecodeRows;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    const int r = warp * kAttnDecodeRows + g + 8 * i;
+#pragma unroll
+    for (int h = 0; h < HD / 8; ++h)
+      *reinterpret_cast<float2*>(po + r * OP + 8 * h + 2 * t) = make_float2(o[h][2 * i], o[h][2 * i + 1]);
+    if (t == 0) {
+      pm[r] = m[i];
+      pl[r] = l[i];
+    }
+  }
+  __syncthreads();
+  constexpr int LANES = HD / 4;  // threads of a row, four values each
+  for (int r = threadIdx.x / LANES; r <= r1 - r0; r += 128 / LANES) {
+    const int c = threadIdx.x % LANES * 4;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, pm[w * kAttnDecodeRows + r]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float total = 0.0f, acc[4] = {};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = exp2_fast(pm[w * kAttnDecodeRows + r] - base);
+      total = fmaf(pl[w * kAttnDecodeRows + r], f, total);
+      const float4 v = *reinterpret_cast<const float4*>(po + (w * kAttnDecodeRows + r) * OP + c);
+      acc[0] = fmaf(v.x, f, acc[0]);
+      acc[1] = fmaf(v.y, f, acc[1]);
+      acc[2] = fmaf(v.z, f, acc[2]);
+      acc[3] = fmaf(v.w, f, acc[3]);
+    }
+    const float inv = total > 0.0f ? 1.0f / total : (total == 0.0f ? 0.0f : total);
+    const float lse2 = total == 0.0f ? -INFINITY : base + log2f(total);
+    const int qi = (r0 + r) / a.G, qh = hk * a.G + (r0 + r) % a.G;
+    const long long head_row = (static_cast<long long>(b) * a.Hq + qh) * a.Lq + qi;
+    if (a.splits > 1) {
+      const long long at = static_cast<long long>(split) * a.B * a.Hq * a.Lq + head_row;
+      if (c == 0) a.part_lse[at] = lse2;
+      if (lse2 != -INFINITY)
+        *reinterpret_cast<float4*>(a.part_o + at * HD + c) = make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+    } else {
+      if (c == 0 && a.lse != nullptr) a.lse[head_row] = lse2 * kLn2;
+      T* out = static_cast<T*>(a.out) + ((static_cast<long long>(b) * a.Lq + qi) * a.Hq + qh) * HD + c;
+      *reinterpret_cast<uint2*>(out) = make_uint2(pack2(acc[0] * inv, acc[1] * inv, T()), pack2(acc[2] * inv, acc[3] * inv, T()));
+    }
+  }
+}
+
 // Joins the partial results of the splits: one warp a (batch, head, query) row.
 template <typename T, int HD>
 __global__ void __launch_bounds__(128) window_attn_join_kernel(const WindowAttnArgs a) {
@@ -327,14 +524,22 @@ __global__ void __launch_bounds__(128) window_attn_join_kernel(const WindowAttnA
   for (int i = 0; i < HD / 32; ++i) out[32 * i] = static_cast<T>(acc[i] * inv);
 }
 
-// Runs a tile's keys are split into: enough tiles to give every SM two CTAs, at least two key tiles a run.
+// The form of a call without tensor-core tiles of queries: rows up to 32 take the single-token kernel (a second tile of
+// 16 rows reads the keys again, from L2), more the one with 64-row tiles.
+inline bool window_attn_decodes(long long rows) { return rows <= 2 * kAttnDecodeRows; }
+
+// Runs the keys of a row tile are split into: enough for four CTAs an SM, none longer than 1024 keys (sequences of
+// unequal lengths share the GPU evenly then), none shorter than two key tiles.
 inline int window_attn_splits(int B, int Lq, int Lk, int Hkv, int G, int window, int sinks, int sm_count) {
-  const long long tiles = (static_cast<long long>(Lq) * G + kAttnRows - 1) / kAttnRows * Hkv * B;
+  const long long rows = static_cast<long long>(Lq) * G;
+  const int per_tile = window_attn_decodes(rows) ? kAttnDecodeRows : kAttnRows;
+  const long long tiles = (rows + per_tile - 1) / per_tile * Hkv * B;
   if (tiles <= 0) return 1;
-  const long long reach = static_cast<long long>(window) + kAttnRows / G + 1;
+  const long long reach = static_cast<long long>(window) + per_tile / G + 1;
   const long long keys = Lk < reach ? Lk : (Lk < reach + sinks ? Lk : reach + sinks);
-  const long long key_tiles = (keys + kAttnBN - 1) / kAttnBN;
-  long long s = (2LL * sm_count + tiles - 1) / tiles;
+  const long long key_tiles = (keys + kAttnBN - 1) / kAttnBN + 1;  // a window need not start at a tile's edge
+  long long s = (4LL * sm_count + tiles - 1) / tiles;
+  if (s < (key_tiles + 15) / 16) s = (key_tiles + 15) / 16;
   if (s > key_tiles / 2) s = key_tiles / 2;
   if (s > 64) s = 64;
   return s < 1 ? 1 : static_cast<int>(s);
@@ -342,13 +547,17 @@ inline int window_attn_splits(int B, int Lq, int Lk, int Hkv, int G, int window,
 
 template <typename T, int HD>
 inline cudaError_t launch_window_attn(const WindowAttnArgs& a, cudaStream_t stream) {
-  constexpr int smem = 4 * kAttnBN * HD * 2;
-  cudaError_t e = cudaFuncSetAttribute(window_attn_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
   const long long rows = static_cast<long long>(a.Lq) * a.G;
-  const dim3 grid(static_cast<unsigned>((rows + kAttnRows - 1) / kAttnRows), static_cast<unsigned>(a.Hkv),
+  const bool decode = window_attn_decodes(rows);
+  constexpr int ring = 4 * kAttnDecodeStages * 2 * 16 * HD * 2, meet = 4 * kAttnDecodeRows * (HD + 8 + 2) * 4;
+  const int smem = decode ? (ring > meet ? ring : meet) : 4 * kAttnBN * HD * 2;
+  const int per_tile = decode ? kAttnDecodeRows : kAttnRows;
+  const auto kernel = decode ? window_attn_decode_kernel<T, HD> : window_attn_kernel<T, HD>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  const dim3 grid(static_cast<unsigned>((rows + per_tile - 1) / per_tile), static_cast<unsigned>(a.Hkv),
                   static_cast<unsigned>(a.B * a.splits));
-  window_attn_kernel<T, HD><<<grid, 128, smem, stream>>>(a);
+  kernel<<<grid, 128, smem, stream>>>(a);
   if (a.splits > 1) {
     const long long total = static_cast<long long>(a.B) * a.Hq * a.Lq;
     window_attn_join_kernel<T, HD><<<static_cast<unsigned>((total + 3) / 4), 128, 0, stream>>>(a);
