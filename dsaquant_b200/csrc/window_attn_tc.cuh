@@ -1,26 +1,27 @@
 // tcgen05 form of the windowed attention, for prompts (see window_attn.cuh for the mathematics).
 //
 // A CTA owns 256 queries of one head as two tiles of 128 rows, A and B, that share every key tile:
-//   warps 0-3    softmax of tile A, one thread a row
-//   warps 4-7    softmax of tile B
-//   warp 8       owns TMEM; one lane issues every MMA
-//   warp 9       TMA producer: Q once, then K and V tiles of 128 keys through one ring
-// TMEM: scores S_A, S_B (128 x 128 fp32 each) and outputs O_A, O_B (128 x HD fp32).  A row's thread reads its
-// 128 scores, and writes its weights P over them as 16-bit pairs: the A operand of the second product
-// comes from TMEM, so the weights never touch shared memory, whose bandwidth the first product needs
-// (both its operands are read from there).
+//   warps 0-7    softmax of tile A, two threads a row (32 keys of each key tile)
+//   warps 8-15   softmax of tile B
+//   warp 16      owns TMEM; one lane of it issues every MMA
+//   warp 17      TMA producer: Q once, then K and V tiles of 64 keys through one ring (warps 18, 19 idle)
+// TMEM: two score buffers a tile (128 x 64 fp32 each) and the outputs O_A, O_B (128 x HD fp32).  A thread reads
+// its 32 scores and writes its weights P over them as 16-bit pairs: the A operand of the second product comes from
+// TMEM, so the weights never touch shared memory, whose bandwidth the first product needs.
 //   S_X(n) = Q_X K(n)^T;   P_X(n) = exp2(S sc - m);   O_X += P_X(n) V(n)
-// The issue order O_A(n), S_A(n+1), O_B(n), S_B(n+1) keeps the tensor pipe on one tile while the other's
-// softmax runs.  S_X(n+1) overwrites P_X(n) behind the product that reads it: MMAs of one thread
-// execute in order.  One commit after S_X(n+1) therefore also says that O_X(n) is complete, which is all the
-// rescaling below needs.
+// S_X(n + 1) is issued before P_X(n) is waited for, into the other buffer, so the softmax warps always find
+// their next scores ready.  (128 keys a tile fill both buffers: a tile's softmax, 2200 cycles, and its products, 1250,
+// then took turns, and the tensor pipe idled 40 % of the time however the softmax was spread over warps.)
+// Four softmax warps on each scheduler hide one another's waits, TMEM accesses and barriers; with two, 64 keys cost 2000
+// cycles a pair of tiles, of which the exponentials are 1024.
+// S_X(n + 2) overwrites P_X(n) behind the product that reads it: MMAs of one thread execute in order.
 //
-// The running maximum m is moved only when a score exceeds it by more than 2^8 (then O and the row sum
-// are rescaled): fp32 sums and 16-bit weights up to 256 lose nothing, and after the first tiles hardly
-// any row moves, so the round trip of O through registers is rare.
+// A row's maximum is found in its first tile and again only when the weights of half a tile add up to over 2^9: until
+// then fp32 sums and 16-bit weights lose nothing by a maximum that is a little old, a tile costs no pass for
+// it, and O is hardly ever rescaled.
 //
-// V rows of keys that no row of the CTA sees are overwritten with zeros in shared memory (tile A's threads,
-// before they hand over P): 0 * garbage must not reach O.  Every wait is bounded.
+// V rows of keys that no row of the CTA sees are overwritten with zeros in shared memory (tile A's threads, before
+// they hand over P): 0 * garbage must not reach O.  Every wait is bounded.
 #pragma once
 #include <cuda.h>
 
@@ -38,18 +39,20 @@ constexpr int kAttnTcMinQueries = 128;
 
 template <int HD>
 struct AttnTcCfg {
-  static constexpr int BM = 128, BN = 128;         // rows of a tile, keys of a tile
-  static constexpr int ATOM = 128 * 128;           // 128 rows of 64 values (one 128-byte swizzle row each)
-  static constexpr int TILE = ATOM * (HD / 64);    // a Q, K or V tile
-  static constexpr int S = HD == 128 ? 5 : 8;      // ring stages
-  static constexpr int OFF_RING = 2 * TILE;
-  static constexpr int OFF_BAR = OFF_RING + S * TILE;
-  // full[S], free[S], q, s[2], p[2], then the abort flag and the TMEM address
-  static constexpr int NUM_BARS = 2 * S + 5;
-  static constexpr int SMEM = OFF_BAR + 8 * NUM_BARS + 16 + 1024;
-  static constexpr int THREADS = 320;
+  static constexpr int BM = 128, BN = 64;            // rows of a tile, keys of a tile
+  static constexpr int Q_ATOM = BM * 128, K_ATOM = BN * 128;  // 64 values of each row (one 128-byte swizzle row each)
+  static constexpr int Q_TILE = Q_ATOM * (HD / 64), K_TILE = K_ATOM * (HD / 64);
+  static constexpr int S = HD == 128 ? 10 : 16;      // ring stages
+  static constexpr int OFF_RING = 2 * Q_TILE;
+  static constexpr int OFF_BAR = OFF_RING + S * K_TILE;
+  // full[S], free[S], q, s[2][2], p[2][2], o[2][2], then the abort flag, the TMEM address and a float a row of both tiles
+  static constexpr int NUM_BARS = 2 * S + 13;
+  static constexpr int OFF_ROWS = OFF_BAR + 8 * NUM_BARS + 16;
+  static constexpr int SMEM = OFF_ROWS + 2 * BM * 4 + 1024;
+  static constexpr int SOFTMAX_WARPS = 16, WARP_MMA = 16, WARP_TMA = 17;
+  static constexpr int THREADS = 640;
   static constexpr int TMEM_COLS = 512;
-  static constexpr int COL_O = 256;                // S at 0 and 128, O at 256 and 256 + HD
+  static constexpr int COL_O = 256;                  // S_A at 0, 64; S_B at 128, 192; O at 256 and 256 + HD
   static_assert(SMEM <= 232448, "shared memory budget");
 };
 
@@ -82,9 +85,30 @@ __host__ __device__ constexpr uint32_t f16_idesc(int n, bool b_mn) {
   return (1u << 4) | (f << 7) | (f << 10) | ((b_mn ? 1u : 0u) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
 }
 
-// Whether rows at positions [p0, p1] see anything of the 128 keys from j0 on.
+// the low n bits, n clamped to 0..32
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Whether rows at positions [p0, p1] see anything of the 64 keys from j0 on.
 __device__ __forceinline__ bool tile_active(int p0, int p1, int j0, int window, int sinks) {
-  return j0 <= p1 && p1 >= 0 && (j0 + 127 > max(p0, 0) - window || j0 < sinks);
+  return j0 <= p1 && p1 >= 0 && (j0 + 63 > max(p0, 0) - window || j0 < sinks);
 }
 
 }  // namespace attn
@@ -99,14 +123,16 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (base - ptx::smem_u32(smem_raw));
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
 
   const uint32_t bar0 = base + C::OFF_BAR;
   auto bar_full = [&](uint32_t s) { return bar0 + 8u * s; };
   auto bar_free = [&](uint32_t s) { return bar0 + 8u * (C::S + s); };
   const uint32_t bar_q = bar0 + 8u * (2 * C::S);
-  auto bar_s = [&](int x) { return bar0 + 8u * (2 * C::S + 1 + x); };
-  auto bar_p = [&](int x) { return bar0 + 8u * (2 * C::S + 3 + x); };
+  auto bar_s = [&](int x, uint32_t buf) { return bar0 + 8u * (2 * C::S + 1 + 2 * x + buf); };
+  // one for each buffer: a warp may be through tile n + 1 before another of its tile is through n
+  auto bar_p = [&](int x, uint32_t buf) { return bar0 + 8u * (2 * C::S + 5 + 2 * x + buf); };
+  auto bar_o = [&](int x, uint32_t buf) { return bar0 + 8u * (2 * C::S + 9 + 2 * x + buf); };
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + C::OFF_BAR + 8 * C::NUM_BARS);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(gen + C::OFF_BAR + 8 * C::NUM_BARS + 8);
   const detail::WaitCtx wctx{abort_flag, prm.status, prm.abort_word, prm.launch_id};
@@ -119,17 +145,21 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     }
     ptx::mbar_init(bar_q, 1);
     for (int x = 0; x < 2; ++x) {
-      ptx::mbar_init(bar_s(x), 1);
-      ptx::mbar_init(bar_p(x), 4);  // one arrival a warp
+      ptx::mbar_init(bar_s(x, 0), 1);
+      ptx::mbar_init(bar_s(x, 1), 1);
+      ptx::mbar_init(bar_p(x, 0), 8);  // one arrival a warp
+      ptx::mbar_init(bar_p(x, 1), 8);
+      ptx::mbar_init(bar_o(x, 0), 1);
+      ptx::mbar_init(bar_o(x, 1), 1);
     }
     *abort_flag = 0;
     ptx::fence_mbar_init();
   }
-  if (warp == 8) {
+  if (warp == C::WARP_MMA) {
     ptx::tmem_alloc<1>(ptx::smem_u32(tmem_holder), C::TMEM_COLS);
     ptx::tmem_relinquish<1>();
   }
-  if (warp == 9 && lane == 0) {
+  if (warp == C::WARP_TMA && lane == 0) {
     ptx::prefetch_tensormap(&tm_q);
     ptx::prefetch_tensormap(&tm_k);
     ptx::prefetch_tensormap(&tm_v);
@@ -137,7 +167,7 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
   ptx::tc_fence_before_sync();
   __syncthreads();
   ptx::tc_fence_after_sync();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_holder);
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t*>(tmem_holder), 0);
 
   // the longest runs (the last queries) first
   const int i0 = static_cast<int>(gridDim.x - 1 - blockIdx.x) * (2 * C::BM);
@@ -148,258 +178,305 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
   // positions of tile x's first and last query (last < first: no queries)
   auto first_pos = [&](int x) { return sp.p0 + x * C::BM; };
   auto last_pos = [&](int x) { return min(sp.p0 + x * C::BM + C::BM - 1, sp.p1); };
-  auto active = [&](int x, int n) {
-    return first_pos(x) <= sp.p1 && tile_active(first_pos(x), last_pos(x), tile_key(n), a.window, a.sinks);
-  };
+  // key tiles that some row of tile x sees: those of the sinks, and [from, to] of the window's (rows are
+  // consecutive, so are these; one more look covers a first window tile that only holds sinks)
+  int from[2], to[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    to[x] = first_pos(x) <= sp.p1 && last_pos(x) >= 0 ? sp.n_sink + last_pos(x) / C::BN - sp.w0 : -1;
+    from[x] = sp.n_sink;
+    while (from[x] <= to[x] && !tile_active(first_pos(x), last_pos(x), tile_key(from[x]), a.window, a.sinks)) ++from[x];
+  }
+  auto active = [&](int x, int n) { return n <= to[x] && (n < sp.n_sink || n >= from[x]); };
 
-  if (warp == 9) {
+  if (warp == C::WARP_TMA) {
     if (lane == 0 && sp.n > 0) {
-      ptx::mbar_arrive_expect_tx(bar_q, 2 * C::TILE);
+      ptx::mbar_arrive_expect_tx(bar_q, 2 * C::Q_TILE);
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int c = 0; c < HD / 64; ++c)
-          ptx::tma_load_4d(base + x * C::TILE + c * C::ATOM, &tm_q, bar_q, 64 * c, hq, i0 + x * C::BM, b);
+#pragma unroll
+          for (int half = 0; half < 2; ++half)  // a box is 64 rows
+            ptx::tma_load_4d(base + x * C::Q_TILE + c * C::Q_ATOM + half * (C::Q_ATOM / 2), &tm_q, bar_q, 64 * c, hq,
+                             i0 + x * C::BM + half * 64, b);
       RingPos<C::S> pos;
-      bool alive = true;
       const int hk = hq / a.G;
-      for (int n = 0; n < sp.n && alive; ++n) {
-        const int j0 = tile_key(n);
+      auto load = [&](const CUtensorMap* map, int n) {
+        if (!wait(bar_free(pos.slot), pos.phase ^ 1)) return false;
+        ptx::mbar_arrive_expect_tx(bar_full(pos.slot), C::K_TILE);
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          if (!wait(bar_free(pos.slot), pos.phase ^ 1)) {
-            alive = false;
-            break;
-          }
-          ptx::mbar_arrive_expect_tx(bar_full(pos.slot), C::TILE);
-#pragma unroll
-          for (int c = 0; c < HD / 64; ++c)
-            ptx::tma_load_4d(base + C::OFF_RING + pos.slot * C::TILE + c * C::ATOM, kv ? &tm_v : &tm_k, bar_full(pos.slot),
-                             64 * c, hk, j0, b);
-          pos.advance();
-        }
-      }
+        for (int c = 0; c < HD / 64; ++c)
+          ptx::tma_load_4d(base + C::OFF_RING + pos.slot * C::K_TILE + c * C::K_ATOM, map, bar_full(pos.slot), 64 * c, hk,
+                           tile_key(n), b);
+        pos.advance();
+        return true;
+      };
+      // in the order of use: K(0), then K(n + 1), V(n)
+      bool alive = load(&tm_k, 0);
+      for (int n = 0; n < sp.n && alive; ++n) alive = (n + 1 == sp.n || load(&tm_k, n + 1)) && load(&tm_v, n);
       if (!alive) {  // loads in flight get a bounded time to land before the block ends
         const uint64_t t0 = ptx::globaltimer_ns();
         while (ptx::globaltimer_ns() - t0 < 2000000ull) {
         }
       }
     }
-  } else if (warp == 8) {
-    if (lane == 0 && sp.n > 0) {
+  } else if (warp == C::WARP_MMA) {
+    if (sp.n > 0) {
+      // the whole warp walks through the loop, one lane's products count
+      const uint32_t one = ptx::elect_one();
       constexpr uint32_t id_s = f16_idesc<T>(C::BN, false), id_o = f16_idesc<T>(HD, true);
-      auto score = [&](int x, uint32_t k_tile) {
-        const uint64_t dq = make_kmajor_sw128_desc(base + x * C::TILE), dk = make_kmajor_sw128_desc(k_tile);
+      // The issuer's instructions are on the critical path: descriptors are split into words, of which only the low
+      // ones (addresses) change, by constants that are known at compile time.
+      const uint64_t dq = make_kmajor_sw128_desc(base), dr = make_kmajor_sw128_desc(base + C::OFF_RING);
+      const uint64_t dv = mn_major_sw128_desc(base + C::OFF_RING, C::K_ATOM);
+      const uint32_t q_lo = static_cast<uint32_t>(dq), k_hi = static_cast<uint32_t>(dr >> 32);
+      const uint32_t r_lo = static_cast<uint32_t>(dr), v_lo0 = static_cast<uint32_t>(dv), v_hi = static_cast<uint32_t>(dv >> 32);
+      uint32_t scored[2] = {0, 0}, done[2] = {0, 0};  // score and output products issued so far
+      auto score = [&](auto xc, uint32_t slot) {
+        constexpr int x = decltype(xc)::value;
+        const uint32_t buf = scored[x]++ & 1, t_s = tmem + x * 128 + buf * C::BN;
+        const uint32_t a_lo = q_lo + x * (C::Q_TILE >> 4), b_lo = r_lo + slot * (C::K_TILE >> 4);
+        ptx::mma_f16_ss<false>(one, t_s, a_lo, k_hi, b_lo, k_hi, id_s);
 #pragma unroll
-        for (int j = 0; j < HD / 16; ++j) {
-          const uint64_t step = (j >> 2) * (C::ATOM >> 4) + (j & 3) * 2;
-          ptx::mma_f16_ss(tmem + x * C::BN, dq + step, dk + step, id_s, j > 0);
-        }
-        ptx::mma_commit(bar_s(x));
+        for (int j = 1; j < HD / 16; ++j)
+          ptx::mma_f16_ss<true>(one, t_s, a_lo + (j >> 2) * (C::Q_ATOM >> 4) + (j & 3) * 2, k_hi,
+                                b_lo + (j >> 2) * (C::K_ATOM >> 4) + (j & 3) * 2, k_hi, id_s);
+        ptx::mma_commit_if(one, bar_s(x, buf));
       };
-      auto output = [&](int x, uint32_t v_tile, bool accumulate) {
-        const uint64_t dv = mn_major_sw128_desc(v_tile, C::ATOM);
+      auto output = [&](auto xc, uint32_t slot) {
+        constexpr int x = decltype(xc)::value;
+        const uint32_t t_p = tmem + x * 128 + (done[x] & 1) * C::BN, b_lo = v_lo0 + slot * (C::K_TILE >> 4);
 #pragma unroll
         for (int j = 0; j < C::BN / 16; ++j)
-          ptx::mma_f16_ts(tmem + C::COL_O + x * HD, tmem + x * C::BN + 8 * j, dv + j * (2048 >> 4), id_o, accumulate || j > 0);
+          ptx::mma_f16_ts(one, tmem + C::COL_O + x * HD, t_p + (j >> 1) * 32 + (j & 1) * 8, b_lo + j * (2048 >> 4), v_hi, id_o,
+                          j > 0 || done[x] > 0 ? 1u : 0u);  // the weights of keys 32.. start at column 32
+        ptx::mma_commit_if(one, bar_o(x, done[x] & 1));
+        ++done[x];
       };
-      auto tile_at = [&](uint32_t slot) { return base + C::OFF_RING + slot * C::TILE; };
+      // The weights are waited for without suspending: the tensor pipe may have nothing else to do.
+      auto wait_soon = [&](uint32_t bar, uint32_t parity) {
+        for (int i = 0; i < 4096; ++i)
+          if (__all_sync(0xffffffffu, ptx::mbar_probe(bar, parity))) return true;
+        return __all_sync(0xffffffffu, wait(bar, parity)) != 0;
+      };
+      auto wait_warp = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+      auto turn = [&](auto xc, int n, uint32_t v_slot) {
+        constexpr int x = decltype(xc)::value;
+        if (!active(x, n)) return true;
+        if (!wait_soon(bar_p(x, done[x] & 1), (done[x] >> 1) & 1)) return false;
+        ptx::tc_fence_after_sync();
+        output(xc, v_slot);
+        return true;
+      };
+      using A = std::integral_constant<int, 0>;
+      using B = std::integral_constant<int, 1>;
       RingPos<C::S> pos;
-      uint32_t p_phase[2] = {0, 0};
-      bool started[2] = {false, false};
-      bool alive = wait(bar_q, 0) && wait(bar_full(0), 0);
-      if (alive) {
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          if (active(x, 0)) score(x, tile_at(0));
-        ptx::mma_commit(bar_free(0));
+      auto scores = [&](int n) {
+        if (!wait_warp(bar_full(pos.slot), pos.phase)) return false;
+        if (active(0, n)) score(A(), pos.slot);
+        if (active(1, n)) score(B(), pos.slot);
+        ptx::mma_commit_if(one, bar_free(pos.slot));
         pos.advance();
-      }
+        return true;
+      };
+      bool alive = wait_warp(bar_q, 0) && scores(0);
       for (int n = 0; n < sp.n && alive; ++n) {
-        const uint32_t v_slot = pos.slot, v_phase = pos.phase;
-        pos.advance();
-        const uint32_t k_slot = pos.slot, k_phase = pos.phase;
-        if (!wait(bar_full(v_slot), v_phase)) {
-          alive = false;
-          break;
-        }
-        bool have_k = false;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          if (active(x, n)) {
-            if (!wait(bar_p(x), p_phase[x])) {
-              alive = false;
-              break;
-            }
-            p_phase[x] ^= 1;
-            ptx::tc_fence_after_sync();
-            output(x, tile_at(v_slot), started[x]);
-            started[x] = true;
-          }
-          if (n + 1 < sp.n) {
-            if (!have_k && !wait(bar_full(k_slot), k_phase)) {
-              alive = false;
-              break;
-            }
-            have_k = true;
-            if (active(x, n + 1)) score(x, tile_at(k_slot));
-          }
-        }
+        alive = (n + 1 == sp.n || scores(n + 1)) && wait_warp(bar_full(pos.slot), pos.phase) && turn(A(), n, pos.slot) &&
+                turn(B(), n, pos.slot);
         if (!alive) break;
-        ptx::mma_commit(bar_free(v_slot));
-        if (n + 1 < sp.n) {
-          ptx::mma_commit(bar_free(k_slot));
-          pos.advance();
-        }
+        ptx::mma_commit_if(one, bar_free(pos.slot));
+        pos.advance();
       }
-      if (alive) {
-        ptx::mma_commit(bar_s(0));  // the outputs are complete
-        ptx::mma_commit(bar_s(1));
-      } else {
+      if (!alive) {
         const uint64_t t0 = ptx::globaltimer_ns();
         while (ptx::globaltimer_ns() - t0 < 2000000ull) {
         }
       }
     }
-  } else {
-    const int x = warp >> 2;
+  } else if (warp < C::SOFTMAX_WARPS) {
+    const int x = warp >> 3, h = (warp >> 2) & 1;   // tile, and half of its keys and of O's columns
     const int r = (warp & 3) * 32 + lane;           // row of the tile = TMEM lane
     const int qi = i0 + x * C::BM + r;
-    const int p = first_pos(x) + r;
+    const int p = min(first_pos(x) + r, sp.p1);     // rows behind the last query see what that one sees
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + lanes + x * C::BN, t_o = tmem + lanes + C::COL_O + x * HD;
-    // the lanes of a warp give up together: the TMEM accesses below want all of them
-    auto wait_all = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+    const uint32_t t_o = tmem + lanes + C::COL_O + x * HD + h * (HD / 2);
+    float* row_float = reinterpret_cast<float*>(gen + C::OFF_ROWS) + x * C::BM + r;
+    // The two warps of the same rows meet at a barrier of their own.  A wait that runs out does not end their loops -
+    // the other warp would wait at the next meeting - they go on to the end (every other wait gives up at
+    // once) and store nothing.
+    const int pair_id = 1 + x * 4 + (warp & 3);
+    auto meet = [&]() { asm volatile("barrier.cta.sync %0, 64;" ::"r"(pair_id) : "memory"); };
+    auto meet_any = [&](bool mine) {
+      uint32_t any;
+      asm volatile(
+          "{\n\t"
+          ".reg .pred p, q;\n\t"
+          "setp.ne.u32 p, %2, 0;\n\t"
+          "barrier.cta.red.or.pred q, %1, 64, p;\n\t"
+          "selp.u32 %0, 1, 0, q;\n\t"
+          "}\n" : "=r"(any) : "r"(pair_id), "r"(static_cast<uint32_t>(mine)) : "memory");
+      return any != 0;
+    };
+    // what both threads of a row know, out of what each knows of its half
+    auto exchange = [&](float v, auto join) {
+      if (h == 0) *row_float = v;
+      meet();
+      if (h == 1) {
+        v = join(*row_float, v);
+        *row_float = v;
+      }
+      meet();
+      return h == 0 ? *row_float : v;
+    };
     const float sc = a.scale * kLog2e;
     const int pa = first_pos(x), pz = last_pos(x);
-    float m = -INFINITY, l = 0.0f;
-    uint32_t s_phase = 0;
-    bool alive = true, started = false;
-    for (int n = 0; n < sp.n && alive; ++n) {
-      const int j0 = tile_key(n);
+    float m = -INFINITY, l = 0.0f;  // the row's maximum, this half's sum
+    uint32_t count = 0;             // tiles this row has been through
+    bool alive = true;
+    for (int n = 0; n < sp.n; ++n) {
       if (!active(x, n)) continue;
-      if (!wait_all(bar_s(x), s_phase)) {
-        alive = false;
-        break;
-      }
-      s_phase ^= 1;
+      const int j0 = tile_key(n);
+      const uint32_t t_s = tmem + lanes + x * 128 + (count & 1) * C::BN + 32 * h;
+      alive &= wait(bar_s(x, count & 1), (count >> 1) & 1);
+      __syncwarp();
       ptx::tc_fence_after_sync();
-      uint32_t s[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32(t_s + 32 * c, s[c]);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) ptx::tmem_ld_wait_for(s[c]);
+      uint32_t s[32];
+      ptx::tmem_ld_32x32(t_s, s);
+      ptx::tmem_ld_wait_for(s);
       const bool whole = j0 + C::BN - 1 <= pa && (j0 > pz - a.window || j0 + C::BN <= a.sinks);
-      if (!whole) {
-        // key j is seen when j <= p and (j > p - window or j < sinks)
-        const int hi = p - j0, lo = p - a.window - j0, first = a.sinks - j0;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int j = 32 * c + i;
-            if (!(j <= hi && (j > lo || j < first))) s[c][i] = 0xff800000u;
-          }
-      }
-      float top = -INFINITY;
-      {
-        float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) t4[i & 3] = fmaxf(t4[i & 3], __uint_as_float(s[c][i]));
-        top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * sc;
-      }
-      // move the maximum only when the weights would pass 2^8
-      const bool move = top > m + 8.0f;
-      if (__any_sync(0xffffffffu, move)) {
-        const float next = move ? top : m;
-        const float f = next == m ? 1.0f : exp2_fast(m - next);  // 0 for a row that starts here
-        m = next;
-        l *= f;
-        if (started) {
+      // A loop of at most one turn: as a plain condition the whole body is predicated and issued for every tile.
 #pragma unroll 1
-          for (int c = 0; c < HD / 32; ++c) {
-            uint32_t o[32];
-            ptx::tmem_ld_32x32(t_o + 32 * c, o);
-            ptx::tmem_ld_wait_for(o);
+      for (bool edge = !whole; edge; edge = false) {
+        // key j is seen when j <= p and (j > p - window or j < sinks)
+        const int j1 = j0 + 32 * h;
+        const uint32_t seen = bits_below(p - j1 + 1) & (~bits_below(p - a.window - j1 + 1) | bits_below(a.sinks - j1));
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            ptx::tmem_st_32x32(t_o + 32 * c, o);
+        for (int i = 0; i < 32; ++i)
+          if (!(seen >> i & 1)) s[i] = 0xff800000u;
+        if (x == 0 || !active(0, n)) {
+          const bool cover = j0 + C::BN - 1 <= sp.hi && (j0 >= sp.lo || j0 + C::BN <= a.sinks);
+          if (!cover) {
+            const uint32_t at = n + 1 < sp.n ? 2 * n + 2 : 2 * n + 1, slot = at % C::S;  // V(n) in the ring
+            const bool here = wait(bar_full(slot), (at / C::S) & 1);
+            alive &= here;
+            const int row = r & 63, j = j0 + row;
+            if (here && !(j <= sp.hi && (j >= sp.lo || j < a.sinks))) {
+#pragma unroll
+              for (int c = 0; c < HD / 64; ++c)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                  detail::sts128(base + C::OFF_RING + slot * C::K_TILE + c * C::K_ATOM + row * 128 +
+                                     16 * (i + 2 * (r >> 6) + 4 * h),
+                                 make_uint4(0, 0, 0, 0));
+            }
+            ptx::fence_proxy_async_smem();
           }
         }
       }
-      started = true;
-      const float neg = m == -INFINITY ? 0.0f : -m;
-      float sum[2] = {0.0f, 0.0f};
+      // Weights against the maximum known so far.  A row that has none yet, or whose weights of this tile add up to
+      // over 2^9 in one half (the only sign that the maximum moved far), makes its warps find the maximum and do
+      // them again.  Only such a row's maximum moves, so what a row gets does not depend on the rows beside it.
+      float sum;
+      bool mine = m == -INFINITY, find = __any_sync(0xffffffffu, mine);  // the same for both halves
+#pragma unroll 1
+      while (true) {
+        if (find) {
+          float top = __uint_as_float(s[0]);  // a NaN score makes it NaN
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+          for (int i = 1; i < 32; ++i) top = detail::max_nan(top, __uint_as_float(s[i]));
+          top = sc * exchange(top, [](float u, float v) { return detail::max_nan(u, v); });
+          const bool move = mine && !(top <= m);
+          const float f = move ? exp2_fast(m - top) : 1.0f;  // 0 for a row that starts here
+          if (move) m = top;
+          l *= f;
+          if (count > 0 && __any_sync(0xffffffffu, move)) {
+            // the product of the tile before has to be in O (the one before that is: these scores came behind it)
+            alive &= wait(bar_o(x, (count - 1) & 1), ((count - 1) >> 1) & 1);
+            __syncwarp();
+            ptx::tc_fence_after_sync();
+#pragma unroll 1
+            for (int c = 0; c < HD / 64; ++c) {
+              uint32_t o[32];
+              ptx::tmem_ld_32x32(t_o + 32 * c, o);
+              ptx::tmem_ld_wait_for(o);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              ptx::tmem_st_32x32(t_o + 32 * c, o);
+            }
+          }
+        }
+        // an infinite maximum leaves no weights: NaN, as inf - inf would
+        const float neg = m == -INFINITY ? 0.0f : (m == INFINITY ? __int_as_float(0x7fc00000) : -m);
+        const uint64_t sc2 = pair(sc, sc), neg2 = pair(neg, neg);
+        uint64_t both = pair(0.0f, 0.0f);
+        // Exponentials run LAG pairs ahead of their sums and conversions: a warp that asks for a result at once
+        // waits out the special-function unit's latency at every pair.
+        constexpr int LAG = 4;
+        float e[32];
         uint32_t w[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float e0 = exp2_fast(fmaf(__uint_as_float(s[c][2 * i]), sc, neg));
-          const float e1 = exp2_fast(fmaf(__uint_as_float(s[c][2 * i + 1]), sc, neg));
-          sum[0] += e0;
-          sum[1] += e1;
-          w[i] = pack2(e0, e1, T());
+        for (int i = 0; i < 16 + LAG; ++i) {
+          if (i < 16) {
+            const uint64_t y = fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), sc2, neg2);
+            float y0, y1;
+            unpair(y, y0, y1);
+            e[2 * i] = exp2_fast(y0);
+            e[2 * i + 1] = exp2_fast(y1);
+          }
+          if (i >= LAG) {
+            const int j = i - LAG;
+            both = add2(both, pair(e[2 * j], e[2 * j + 1]));
+            w[j] = pack2(e[2 * j], e[2 * j + 1], T());
+          }
         }
-        ptx::tmem_st_32x16(t_s + 16 * c, w);
+        ptx::tmem_st_32x16(t_s, w);
+        float sum1;
+        unpair(both, sum, sum1);
+        sum += sum1;
+        const bool bad = !mine && !(sum <= 512.0f);  // a row that just moved has weights of at most 1
+        find = meet_any(bad);
+        if (!find) break;
+        mine = exchange(bad ? 1.0f : 0.0f, [](float u, float v) { return fmaxf(u, v); }) != 0.0f;
+        meet();
+        ptx::tmem_st_wait();  // the weights are written again
       }
-      l += sum[0] + sum[1];
+      l += sum;
       ptx::tmem_st_wait();
-      if (x == 0 || !active(0, n)) {
-        const bool cover = j0 + C::BN - 1 <= sp.hi && (j0 >= sp.lo || j0 + C::BN <= a.sinks);
-        if (!cover) {
-          // V(n) follows K(n) in the ring
-          const uint32_t at = 2 * n + 1, slot = at % C::S;
-          if (!wait_all(bar_full(slot), (at / C::S) & 1)) {
-            alive = false;
-            break;
-          }
-          const int j = j0 + r;
-          if (!(j <= sp.hi && (j >= sp.lo || j < a.sinks))) {
-#pragma unroll
-            for (int c = 0; c < HD / 64; ++c)
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                detail::sts128(base + C::OFF_RING + slot * C::TILE + c * C::ATOM + r * 128 + 16 * i, make_uint4(0, 0, 0, 0));
-          }
-          ptx::fence_proxy_async_smem();
-        }
-      }
       ptx::tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(bar_p(x));
+      if (lane == 0) ptx::mbar_arrive(bar_p(x, count & 1));
+      ++count;
     }
-    if (alive && sp.n > 0) {
-      alive = wait_all(bar_s(x), s_phase);
+    if (count > 0) {
+      alive &= wait(bar_o(x, (count - 1) & 1), ((count - 1) >> 1) & 1);
+      __syncwarp();
       ptx::tc_fence_after_sync();
     }
-    if (alive) {
-      const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-      const bool ok = qi < a.Lq;
-      if (ok && a.lse != nullptr)
-        a.lse[(static_cast<long long>(b) * a.Hq + hq) * a.Lq + qi] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
-      T* out = static_cast<T*>(a.out) + ((static_cast<long long>(b) * a.Lq + qi) * a.Hq + hq) * HD;
+    l = exchange(l, [](float u, float v) { return u + v; });
+    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+    const bool ok = qi < a.Lq && alive;
+    if (h == 0 && ok && a.lse != nullptr)
+      a.lse[(static_cast<long long>(b) * a.Hq + hq) * a.Lq + qi] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+    T* out = static_cast<T*>(a.out) + ((static_cast<long long>(b) * a.Lq + qi) * a.Hq + hq) * HD + h * (HD / 2);
 #pragma unroll 1
-      for (int c = 0; c < HD / 32; ++c) {
-        uint32_t o[32];
-        if (started) {  // the same for the whole warp
-          ptx::tmem_ld_32x32(t_o + 32 * c, o);
-          ptx::tmem_ld_wait_for(o);
-        } else {
+    for (int c = 0; c < HD / 64; ++c) {
+      uint32_t o[32];
+      if (count > 0) {  // the same for the whole warp
+        ptx::tmem_ld_32x32(t_o + 32 * c, o);
+        ptx::tmem_ld_wait_for(o);
+      } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0u;
-        }
-        if (ok) {
+        for (int i = 0; i < 32; ++i) o[i] = 0u;
+      }
+      if (ok) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t w[4];
+        for (int i = 0; i < 4; ++i) {
+          uint32_t v[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              w[j] = pack2(__uint_as_float(o[8 * i + 2 * j]) * inv, __uint_as_float(o[8 * i + 2 * j + 1]) * inv, T());
-            *reinterpret_cast<uint4*>(out + 32 * c + 8 * i) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
+          for (int j = 0; j < 4; ++j)
+            v[j] = pack2(__uint_as_float(o[8 * i + 2 * j]) * inv, __uint_as_float(o[8 * i + 2 * j + 1]) * inv, T());
+          *reinterpret_cast<uint4*>(out + 32 * c + 8 * i) = make_uint4(v[0], v[1], v[2], v[3]);
         }
       }
     }
@@ -407,14 +484,14 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
 
   ptx::tc_fence_before_sync();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == C::WARP_MMA) {
     __syncwarp();
     ptx::tc_fence_after_sync();
     ptx::tmem_dealloc<1>(tmem, C::TMEM_COLS);
   }
 }
 
-// [batch, token, head, HD] as a 4-D map (HD, head, token, batch) with boxes of 64 values x 128 tokens.
+// [batch, token, head, HD] as a 4-D map (HD, head, token, batch) with boxes of 64 values x 64 tokens.
 inline int encode_attn_map(CUtensorMap* map, bool bf16, const void* base, int hd, int heads, int tokens, int batch,
                            long long p_head, long long p_tok, long long p_batch) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -428,7 +505,7 @@ inline int encode_attn_map(CUtensorMap* map, bool bf16, const void* base, int hd
   const cuuint64_t strides[3] = {heads > 1 ? static_cast<cuuint64_t>(2 * p_head) : 256u,
                                  tokens > 1 ? static_cast<cuuint64_t>(2 * p_tok) : 256u,
                                  batch > 1 ? static_cast<cuuint64_t>(2 * p_batch) : 256u};
-  const cuuint32_t box[4] = {64, 1, 128, 1}, one[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, 1, 64, 1}, one[4] = {1, 1, 1, 1};
   const CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
                          const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
