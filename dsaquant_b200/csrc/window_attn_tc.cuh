@@ -3,8 +3,8 @@
 // A CTA owns 256 queries of one head as two tiles of 128 rows, A and B, that share every key tile:
 //   warps 0-7    softmax of tile A, two threads a row (32 keys of each key tile)
 //   warps 8-15   softmax of tile B
-//   warp 16      owns TMEM; one lane of it issues every MMA
-//   warp 17      TMA producer: Q once, then K and V tiles of 64 keys through one ring (warps 18, 19 idle)
+//   warps 16, 17 one lane of each issues the MMAs of tile A, of tile B; warp 16 owns TMEM
+//   warp 18      TMA producer: Q once, then K and V tiles of 64 keys through one ring (warp 19 idles)
 // TMEM: two score buffers a tile (128 x 64 fp32 each) and the outputs O_A, O_B (128 x HD fp32).  A thread reads
 // its 32 scores and writes its weights P over them as 16-bit pairs: the A operand of the second product comes from
 // TMEM, so the weights never touch shared memory, whose bandwidth the first product needs.
@@ -14,14 +14,16 @@
 // then took turns, and the tensor pipe idled 40 % of the time however the softmax was spread over warps.)
 // Four softmax warps on each scheduler hide one another's waits, TMEM accesses and barriers; with two, 64 keys cost 2000
 // cycles a pair of tiles, of which the exponentials are 1024.
+// An issuer's waits and commits take as long as its products (830 of 1800 cycles when one warp did both tiles); with
+// two, one tile's products fill the pipe meanwhile.
 // S_X(n + 2) overwrites P_X(n) behind the product that reads it: MMAs of one thread execute in order.
 //
 // A row's maximum is found in its first tile and again only when the weights of half a tile add up to over 2^9: until
 // then fp32 sums and 16-bit weights lose nothing by a maximum that is a little old, a tile costs no pass for
 // it, and O is hardly ever rescaled.
 //
-// V rows of keys that no row of the CTA sees are overwritten with zeros in shared memory (tile A's threads, before
-// they hand over P): 0 * garbage must not reach O.  Every wait is bounded.
+// V rows of keys that no row of the CTA sees are overwritten with zeros in shared memory (by each tile's threads,
+// before they hand over P): 0 * garbage must not reach O.  Every wait is bounded.
 #pragma once
 #include <cuda.h>
 
@@ -49,7 +51,7 @@ struct AttnTcCfg {
   static constexpr int NUM_BARS = 2 * S + 13;
   static constexpr int OFF_ROWS = OFF_BAR + 8 * NUM_BARS + 16;
   static constexpr int SMEM = OFF_ROWS + 2 * BM * 4 + 1024;
-  static constexpr int SOFTMAX_WARPS = 16, WARP_MMA = 16, WARP_TMA = 17;
+  static constexpr int SOFTMAX_WARPS = 16, WARP_MMA = 16, WARP_TMA = 18;
   static constexpr int THREADS = 640;
   static constexpr int TMEM_COLS = 512;
   static constexpr int COL_O = 256;                  // S_A at 0, 64; S_B at 128, 192; O at 256 and 256 + HD
@@ -141,7 +143,7 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::S; ++s) {
       ptx::mbar_init(bar_full(s), 1);
-      ptx::mbar_init(bar_free(s), 1);
+      ptx::mbar_init(bar_free(s), 2);  // both issuers
     }
     ptx::mbar_init(bar_q, 1);
     for (int x = 0; x < 2; ++x) {
@@ -180,14 +182,19 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
   auto last_pos = [&](int x) { return min(sp.p0 + x * C::BM + C::BM - 1, sp.p1); };
   // key tiles that some row of tile x sees: those of the sinks, and [from, to] of the window's (rows are
   // consecutive, so are these; one more look covers a first window tile that only holds sinks)
-  int from[2], to[2];
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    to[x] = first_pos(x) <= sp.p1 && last_pos(x) >= 0 ? sp.n_sink + last_pos(x) / C::BN - sp.w0 : -1;
-    from[x] = sp.n_sink;
-    while (from[x] <= to[x] && !tile_active(first_pos(x), last_pos(x), tile_key(from[x]), a.window, a.sinks)) ++from[x];
-  }
-  auto active = [&](int x, int n) { return n <= to[x] && (n < sp.n_sink || n >= from[x]); };
+  auto last_tile = [&](int x) {
+    return first_pos(x) <= sp.p1 && last_pos(x) >= 0 ? sp.n_sink + last_pos(x) / C::BN - sp.w0 : -1;
+  };
+  auto first_tile = [&](int x, int last) {
+    int n = sp.n_sink;
+    while (n <= last && !tile_active(first_pos(x), last_pos(x), tile_key(n), a.window, a.sinks)) ++n;
+    return n;
+  };
+  const int to_a = last_tile(0), to_b = last_tile(1), from_a = first_tile(0, to_a), from_b = first_tile(1, to_b);
+  auto active = [&](int x, int n) {
+    const int to = x == 0 ? to_a : to_b, from = x == 0 ? from_a : from_b;
+    return n <= to && (n < sp.n_sink || n >= from);
+  };
 
   if (warp == C::WARP_TMA) {
     if (lane == 0 && sp.n > 0) {
@@ -221,73 +228,62 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         }
       }
     }
-  } else if (warp == C::WARP_MMA) {
+  } else if (warp == C::WARP_MMA || warp == C::WARP_MMA + 1) {
     if (sp.n > 0) {
       // the whole warp walks through the loop, one lane's products count
       const uint32_t one = ptx::elect_one();
+      const int x = warp - C::WARP_MMA;
       constexpr uint32_t id_s = f16_idesc<T>(C::BN, false), id_o = f16_idesc<T>(HD, true);
       // The issuer's instructions are on the critical path: descriptors are split into words, of which only the low
       // ones (addresses) change, by constants that are known at compile time.
-      const uint64_t dq = make_kmajor_sw128_desc(base), dr = make_kmajor_sw128_desc(base + C::OFF_RING);
+      const uint64_t dq = make_kmajor_sw128_desc(base + x * C::Q_TILE), dr = make_kmajor_sw128_desc(base + C::OFF_RING);
       const uint64_t dv = mn_major_sw128_desc(base + C::OFF_RING, C::K_ATOM);
-      const uint32_t q_lo = static_cast<uint32_t>(dq), k_hi = static_cast<uint32_t>(dr >> 32);
+      const uint32_t a_lo = static_cast<uint32_t>(dq), k_hi = static_cast<uint32_t>(dr >> 32);
       const uint32_t r_lo = static_cast<uint32_t>(dr), v_lo0 = static_cast<uint32_t>(dv), v_hi = static_cast<uint32_t>(dv >> 32);
-      uint32_t scored[2] = {0, 0}, done[2] = {0, 0};  // score and output products issued so far
-      auto score = [&](auto xc, uint32_t slot) {
-        constexpr int x = decltype(xc)::value;
-        const uint32_t buf = scored[x]++ & 1, t_s = tmem + x * 128 + buf * C::BN;
-        const uint32_t a_lo = q_lo + x * (C::Q_TILE >> 4), b_lo = r_lo + slot * (C::K_TILE >> 4);
-        ptx::mma_f16_ss<false>(one, t_s, a_lo, k_hi, b_lo, k_hi, id_s);
-#pragma unroll
-        for (int j = 1; j < HD / 16; ++j)
-          ptx::mma_f16_ss<true>(one, t_s, a_lo + (j >> 2) * (C::Q_ATOM >> 4) + (j & 3) * 2, k_hi,
-                                b_lo + (j >> 2) * (C::K_ATOM >> 4) + (j & 3) * 2, k_hi, id_s);
-        ptx::mma_commit_if(one, bar_s(x, buf));
-      };
-      auto output = [&](auto xc, uint32_t slot) {
-        constexpr int x = decltype(xc)::value;
-        const uint32_t t_p = tmem + x * 128 + (done[x] & 1) * C::BN, b_lo = v_lo0 + slot * (C::K_TILE >> 4);
-#pragma unroll
-        for (int j = 0; j < C::BN / 16; ++j)
-          ptx::mma_f16_ts(one, tmem + C::COL_O + x * HD, t_p + (j >> 1) * 32 + (j & 1) * 8, b_lo + j * (2048 >> 4), v_hi, id_o,
-                          j > 0 || done[x] > 0 ? 1u : 0u);  // the weights of keys 32.. start at column 32
-        ptx::mma_commit_if(one, bar_o(x, done[x] & 1));
-        ++done[x];
-      };
+      const uint32_t t_x = tmem + x * 128, t_o = tmem + C::COL_O + x * HD;
+      uint32_t scored = 0, done = 0;  // score and output products issued so far
+      auto wait_warp = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
       // The weights are waited for without suspending: the tensor pipe may have nothing else to do.
       auto wait_soon = [&](uint32_t bar, uint32_t parity) {
         for (int i = 0; i < 4096; ++i)
           if (__all_sync(0xffffffffu, ptx::mbar_probe(bar, parity))) return true;
-        return __all_sync(0xffffffffu, wait(bar, parity)) != 0;
+        return wait_warp(bar, parity);
       };
-      auto wait_warp = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
-      auto turn = [&](auto xc, int n, uint32_t v_slot) {
-        constexpr int x = decltype(xc)::value;
-        if (!active(x, n)) return true;
-        if (!wait_soon(bar_p(x, done[x] & 1), (done[x] >> 1) & 1)) return false;
-        ptx::tc_fence_after_sync();
-        output(xc, v_slot);
-        return true;
-      };
-      using A = std::integral_constant<int, 0>;
-      using B = std::integral_constant<int, 1>;
       RingPos<C::S> pos;
       auto scores = [&](int n) {
         if (!wait_warp(bar_full(pos.slot), pos.phase)) return false;
-        if (active(0, n)) score(A(), pos.slot);
-        if (active(1, n)) score(B(), pos.slot);
+        if (active(x, n)) {
+          const uint32_t buf = scored++ & 1, t_s = t_x + buf * C::BN, b_lo = r_lo + pos.slot * (C::K_TILE >> 4);
+          ptx::mma_f16_ss<false>(one, t_s, a_lo, k_hi, b_lo, k_hi, id_s);
+#pragma unroll
+          for (int j = 1; j < HD / 16; ++j)
+            ptx::mma_f16_ss<true>(one, t_s, a_lo + (j >> 2) * (C::Q_ATOM >> 4) + (j & 3) * 2, k_hi,
+                                  b_lo + (j >> 2) * (C::K_ATOM >> 4) + (j & 3) * 2, k_hi, id_s);
+          ptx::mma_commit_if(one, bar_s(x, buf));
+        }
+        ptx::mma_commit_if(one, bar_free(pos.slot));
+        pos.advance();
+        return true;
+      };
+      auto output = [&](int n) {
+        if (!wait_warp(bar_full(pos.slot), pos.phase)) return false;
+        if (active(x, n)) {
+          const uint32_t buf = done & 1, t_p = t_x + buf * C::BN, b_lo = v_lo0 + pos.slot * (C::K_TILE >> 4);
+          if (!wait_soon(bar_p(x, buf), (done >> 1) & 1)) return false;
+          ptx::tc_fence_after_sync();
+#pragma unroll
+          for (int j = 0; j < C::BN / 16; ++j)
+            ptx::mma_f16_ts(one, t_o, t_p + (j >> 1) * 32 + (j & 1) * 8, b_lo + j * (2048 >> 4), v_hi, id_o,
+                            j > 0 || done > 0 ? 1u : 0u);  // the weights of keys 32.. start at column 32
+          ptx::mma_commit_if(one, bar_o(x, buf));
+          ++done;
+        }
         ptx::mma_commit_if(one, bar_free(pos.slot));
         pos.advance();
         return true;
       };
       bool alive = wait_warp(bar_q, 0) && scores(0);
-      for (int n = 0; n < sp.n && alive; ++n) {
-        alive = (n + 1 == sp.n || scores(n + 1)) && wait_warp(bar_full(pos.slot), pos.phase) && turn(A(), n, pos.slot) &&
-                turn(B(), n, pos.slot);
-        if (!alive) break;
-        ptx::mma_commit_if(one, bar_free(pos.slot));
-        pos.advance();
-      }
+      for (int n = 0; n < sp.n && alive; ++n) alive = (n + 1 == sp.n || scores(n + 1)) && output(n);
       if (!alive) {
         const uint64_t t0 = ptx::globaltimer_ns();
         while (ptx::globaltimer_ns() - t0 < 2000000ull) {
@@ -354,24 +350,22 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
 #pragma unroll
         for (int i = 0; i < 32; ++i)
           if (!(seen >> i & 1)) s[i] = 0xff800000u;
-        if (x == 0 || !active(0, n)) {
-          const bool cover = j0 + C::BN - 1 <= sp.hi && (j0 >= sp.lo || j0 + C::BN <= a.sinks);
-          if (!cover) {
-            const uint32_t at = n + 1 < sp.n ? 2 * n + 2 : 2 * n + 1, slot = at % C::S;  // V(n) in the ring
-            const bool here = wait(bar_full(slot), (at / C::S) & 1);
-            alive &= here;
-            const int row = r & 63, j = j0 + row;
-            if (here && !(j <= sp.hi && (j >= sp.lo || j < a.sinks))) {
+        const bool cover = j0 + C::BN - 1 <= sp.hi && (j0 >= sp.lo || j0 + C::BN <= a.sinks);
+        if (!cover) {
+          const uint32_t at = n + 1 < sp.n ? 2 * n + 2 : 2 * n + 1, slot = at % C::S;  // V(n) in the ring
+          const bool here = wait(bar_full(slot), (at / C::S) & 1);
+          alive &= here;
+          const int row = r & 63, j = j0 + row;
+          if (here && !(j <= sp.hi && (j >= sp.lo || j < a.sinks))) {
 #pragma unroll
-              for (int c = 0; c < HD / 64; ++c)
+            for (int c = 0; c < HD / 64; ++c)
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                  detail::sts128(base + C::OFF_RING + slot * C::K_TILE + c * C::K_ATOM + row * 128 +
-                                     16 * (i + 2 * (r >> 6) + 4 * h),
-                                 make_uint4(0, 0, 0, 0));
-            }
-            ptx::fence_proxy_async_smem();
+              for (int i = 0; i < 2; ++i)
+                detail::sts128(base + C::OFF_RING + slot * C::K_TILE + c * C::K_ATOM + row * 128 +
+                                   16 * (i + 2 * (r >> 6) + 4 * h),
+                               make_uint4(0, 0, 0, 0));
           }
+          ptx::fence_proxy_async_smem();
         }
       }
       // Weights against the maximum known so far.  A row that has none yet, or whose weights of this tile add up to
