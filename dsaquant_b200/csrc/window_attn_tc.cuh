@@ -108,6 +108,13 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+// The waiting part of a bounded wait, out of line: the roles' loops share the instruction caches.
+__device__ __noinline__ bool wait_longer(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status,
+                                         unsigned* abort_word, unsigned launch_id) {
+  return b200w4a4::detail::wait_bar(bar, parity, b200w4a4::detail::WaitCtx{abort_flag, status, abort_word, launch_id},
+                                    DEV_TIMEOUT_ATTENTION);
+}
+
 // Whether rows at positions [p0, p1] see anything of the 64 keys from j0 on.
 __device__ __forceinline__ bool tile_active(int p0, int p1, int j0, int window, int sinks) {
   return j0 <= p1 && p1 >= 0 && (j0 + 63 > max(p0, 0) - window || j0 < sinks);
@@ -137,8 +144,9 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
   auto bar_o = [&](int x, uint32_t buf) { return bar0 + 8u * (2 * C::S + 9 + 2 * x + buf); };
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + C::OFF_BAR + 8 * C::NUM_BARS);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(gen + C::OFF_BAR + 8 * C::NUM_BARS + 8);
-  const detail::WaitCtx wctx{abort_flag, prm.status, prm.abort_word, prm.launch_id};
-  auto wait = [&](uint32_t bar, uint32_t parity) { return detail::wait_bar(bar, parity, wctx, DEV_TIMEOUT_ATTENTION); };
+  auto wait = [&](uint32_t bar, uint32_t parity) {
+    return ptx::mbar_probe(bar, parity) || wait_longer(bar, parity, abort_flag, prm.status, prm.abort_word, prm.launch_id);
+  };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::S; ++s) {
