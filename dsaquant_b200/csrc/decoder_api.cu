@@ -52,6 +52,7 @@ int b200w4a4_rms_norm_quant(const void* x, int x_dtype, long long x_ld, const vo
   if (M < 0 || D < 1 || D > kRmsNormMaxD) return B200W4A4_ESHAPE;
   if (M == 0) return B200W4A4_OK;
   if (x == nullptr || weight == nullptr || codes == nullptr || scale == nullptr) return B200W4A4_EINVAL;
+  if (residual_out != nullptr && (residual_out == x || residual_out == residual)) return B200W4A4_EINVAL;
   if ((M > 1 && x_ld < D) || (residual != nullptr && M > 1 && residual_ld < D)) return B200W4A4_ESHAPE;
   const unsigned es = size_of(x_dtype);
   if (!aligned(x, es) || !aligned(residual, es) || !aligned(residual_out, es) || !aligned(weight, size_of(w_dtype)) ||

@@ -6,6 +6,11 @@
 // The row is loaded once and stays in registers as fp32 through both reductions (sum of squares,
 // abs-max), so what moves is x, the residual in and out, one byte a value and four a row.
 //
+// e4m3 codes are those of the exact quotient: its midpoints are 2^-4 of a value apart, so among millions of values
+// some always lie within the fp32 roundings of one, and a code on the wrong side is a step of 6 %.  A value whose
+// quotient lies within 16 fp32 steps of a midpoint (one in 2^15) is read again and decided in 64 bits, against the
+// row's largest |s * weight|, of which 64 bits are kept too; the rsqrt cancels.
+//
 // A row whose sum of squares or whose y is not finite has no meaningful codes: its scale is NaN
 // (whatever is computed from it shows it) and its codes are 0.
 #pragma once
@@ -84,8 +89,18 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 __device__ __forceinline__ uint32_t code_int8(float y, float inv) {
   return __float_as_uint(fminf(fmaxf(y * inv, -128.0f), 127.0f) + kRoundMagic);  // low byte
 }
-__device__ __forceinline__ uint32_t code_e4m3x2(float lo, float hi, float inv) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(lo * inv, hi * inv), __NV_SATFINITE, __NV_E4M3);
+// distance of a positive quotient's bits from the first pattern 16 steps below an e4m3 midpoint: under 32 near one
+__device__ __forceinline__ uint32_t past_midpoint(float t) { return (__float_as_uint(t) - 0x7fff0u) & 0xfffffu; }
+// the e4m3 value nearest to num / den (den > 0), a quotient near a midpoint; compared without dividing, so ties are seen
+__device__ __forceinline__ float nearest_e4m3(double num, double den) {
+  const float t = static_cast<float>(fabs(num) / den);
+  const uint32_t low = (__float_as_uint(t) - 32u) & 0xfff00000u;  // the lower neighbour
+  const double mid = static_cast<double>(__uint_as_float(low | 0x80000u)) * den, a = fabs(num);
+  const bool up = a > mid || (a == mid && (low & 0x100000u) != 0);  // ties to the even one
+  return copysignf(__uint_as_float(up ? low + 0x100000u : low), static_cast<float>(num));
+}
+__device__ __forceinline__ uint32_t code_e4m3x2(float lo, float hi) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
 
 }  // namespace detail
@@ -93,10 +108,11 @@ __device__ __forceinline__ uint32_t code_e4m3x2(float lo, float hi, float inv) {
 // TPR threads share a row and hold NCH * 8 of its values each.  VEC: eight consecutive values a
 // chunk, moved with 128-bit accesses (D, pitches and addresses allow it).  Otherwise a chunk is
 // eight values TPR apart and every access moves one value, coalesced across the threads.
-template <typename T, int TPR, int NCH, bool VEC>
-__global__ void __launch_bounds__(256) rms_norm_quant_kernel(const RmsNormArgs a) {
+template <typename T, int TPR, int NCH, bool VEC, bool E4M3>
+__global__ void __launch_bounds__(256, NCH <= 5 ? 4 : 2) rms_norm_quant_kernel(const RmsNormArgs a) {
   constexpr int ROWS = 256 / TPR;
   __shared__ float red[2][8];
+  __shared__ unsigned long long top64[8];  // a row's largest |s * weight| in 64 bits (e4m3)
   const int sub = threadIdx.x / TPR;
   const int t = threadIdx.x % TPR;
   const long long row = static_cast<long long>(blockIdx.x) * ROWS + sub;
@@ -105,6 +121,7 @@ __global__ void __launch_bounds__(256) rms_norm_quant_kernel(const RmsNormArgs a
   const T* rr = static_cast<const T*>(a.residual);
   if (rr != nullptr) rr += (row_ok ? row : 0) * a.r_ld;
   T* ro = static_cast<T*>(a.residual_out) + row * a.D;
+  if (threadIdx.x < ROWS) top64[threadIdx.x] = 0ull;
   auto at = [&](int i, int e) { return VEC ? 8 * (t + i * TPR) + e : (8 * i + e) * TPR + t; };
 
   float v[NCH][8];
@@ -142,13 +159,16 @@ __global__ void __launch_bounds__(256) rms_norm_quant_kernel(const RmsNormArgs a
       for (int e = 0; e < 8; ++e) v[i][e] = row_ok && at(i, e) < a.D ? detail::load_f32(xr + at(i, e)) : 0.0f;
     if (rr != nullptr && row_ok) {
 #pragma unroll
-      for (int i = 0; i < NCH; ++i)
+      for (int i = 0; i < NCH; ++i) {
+        float r[8];  // the residual may be overwritten: a chunk's loads come before its stores
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (at(i, e) < a.D) {
-            v[i][e] += detail::load_f32(rr + at(i, e));
-            detail::store_f32(ro + at(i, e), v[i][e]);
-          }
+        for (int e = 0; e < 8; ++e) r[e] = at(i, e) < a.D ? detail::load_f32(rr + at(i, e)) : 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[i][e] += r[e];
+          if (at(i, e) < a.D) detail::store_f32(ro + at(i, e), v[i][e]);
+        }
+      }
     }
   }
 #pragma unroll
@@ -159,97 +179,134 @@ __global__ void __launch_bounds__(256) rms_norm_quant_kernel(const RmsNormArgs a
   const float rstd = rsqrtf(ss / static_cast<float>(a.D) + a.eps);
 
   float amax = 0.0f;
+  auto normalise = [&](const auto* weight) {
 #pragma unroll
-  for (int i = 0; i < NCH; ++i) {
-    float w[8];
-    if constexpr (VEC) {
-      if (at(i, 0) < a.D) {
-        if (a.w_dtype == XDT_F16) detail::weight8(static_cast<const __half*>(a.weight) + at(i, 0), w);
-        else if (a.w_dtype == XDT_BF16) detail::weight8(static_cast<const __nv_bfloat16*>(a.weight) + at(i, 0), w);
-        else detail::weight8(static_cast<const float*>(a.weight) + at(i, 0), w);
+    for (int i = 0; i < NCH; ++i) {
+      float w[8];
+      if constexpr (VEC) {
+        if (at(i, 0) >= a.D) continue;  // zeros
+        detail::weight8(weight + at(i, 0), w);
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = 0.0f;
+        for (int e = 0; e < 8; ++e) w[e] = at(i, e) < a.D ? detail::load_f32(weight + at(i, e)) : 0.0f;
       }
-    } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int c = at(i, e);
-        w[e] = 0.0f;
-        if (c < a.D) {
-          if (a.w_dtype == XDT_F16) w[e] = detail::load_f32(static_cast<const __half*>(a.weight) + c);
-          else if (a.w_dtype == XDT_BF16) w[e] = detail::load_f32(static_cast<const __nv_bfloat16*>(a.weight) + c);
-          else w[e] = detail::load_f32(static_cast<const float*>(a.weight) + c);
-        }
+        v[i][e] = v[i][e] * rstd * w[e];
+        amax = detail::max_nan(amax, fabsf(v[i][e]));
       }
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      v[i][e] = v[i][e] * rstd * w[e];
-      amax = detail::max_nan(amax, fabsf(v[i][e]));
-    }
-  }
+  };
+  if (a.w_dtype == XDT_F16) normalise(static_cast<const __half*>(a.weight));
+  else if (a.w_dtype == XDT_BF16) normalise(static_cast<const __nv_bfloat16*>(a.weight));
+  else normalise(static_cast<const float*>(a.weight));
   // a NaN must survive the reduction too: it travels as +inf, which no finite row reaches
   if (!(amax < INFINITY)) amax = INFINITY;
   amax = row_reduce<TPR, true>(amax, red[1], sub);
-  if (!row_ok) return;
   const bool good = ss < INFINITY && amax < INFINITY;  // false for NaN
-  const float top = a.format == CODES_INT8 ? 127.0f : 448.0f;
+  const float top = E4M3 ? 448.0f : 127.0f;
   const float s = __fmul_rn(__fdiv_rn(fmaxf(amax, 1e-5f), top), a.clip);
-  if (t == 0) a.scale[row] = good ? s : __int_as_float(0x7fc00000);
   const float inv = __fdiv_rn(1.0f, s);
-  uint8_t* q = static_cast<uint8_t*>(a.codes) + row * a.D;
+  uint8_t* q = static_cast<uint8_t*>(a.codes) + (row_ok ? row : 0) * a.D;
+  // e4m3: which of this thread's values are the row's largest, and which lie near a midpoint
+  constexpr int MW = E4M3 ? (NCH + 3) / 4 : 1;
+  uint32_t largest[MW] = {}, near[MW] = {};
+  if constexpr (E4M3) {
+#pragma unroll
+    for (int i = 0; i < NCH; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (fabsf(v[i][e]) == amax) largest[i / 4] |= 1u << (8 * (i % 4) + e);
+        v[i][e] = fminf(fmaxf(v[i][e] * inv, -448.0f), 448.0f);
+        if (detail::past_midpoint(v[i][e]) < 32) near[i / 4] |= 1u << (8 * (i % 4) + e);
+      }
+  }
+  if (row_ok && t == 0) a.scale[row] = good ? s : __int_as_float(0x7fc00000);
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
     if constexpr (VEC) {
       if (at(i, 0) >= a.D) continue;
       uint2 o = make_uint2(0u, 0u);
       if (good) {
-        if (a.format == CODES_INT8) {
+        if constexpr (E4M3) {
+          o.x = detail::code_e4m3x2(v[i][0], v[i][1]) | detail::code_e4m3x2(v[i][2], v[i][3]) << 16;
+          o.y = detail::code_e4m3x2(v[i][4], v[i][5]) | detail::code_e4m3x2(v[i][6], v[i][7]) << 16;
+        } else {
           uint32_t c[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) c[e] = detail::code_int8(v[i][e], inv);
           o.x = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
           o.y = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
-        } else {
-          o.x = detail::code_e4m3x2(v[i][0], v[i][1], inv) | detail::code_e4m3x2(v[i][2], v[i][3], inv) << 16;
-          o.y = detail::code_e4m3x2(v[i][4], v[i][5], inv) | detail::code_e4m3x2(v[i][6], v[i][7], inv) << 16;
         }
       }
-      *reinterpret_cast<uint2*>(q + at(i, 0)) = o;
+      if (row_ok) *reinterpret_cast<uint2*>(q + at(i, 0)) = o;
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         if (at(i, e) >= a.D) continue;
         uint32_t c = 0;
-        if (good)
-          c = a.format == CODES_INT8 ? detail::code_int8(v[i][e], inv) : detail::code_e4m3x2(v[i][e], 0.0f, inv);
-        q[at(i, e)] = static_cast<uint8_t>(c);
+        if (good) c = E4M3 ? detail::code_e4m3x2(v[i][e], 0.0f) : detail::code_int8(v[i][e], inv);
+        if (row_ok) q[at(i, e)] = static_cast<uint8_t>(c);
       }
     }
+  }
+  if constexpr (E4M3) {
+    auto product64 = [&](int c) {  // s * weight of one value, read again
+      double s64 = static_cast<double>(detail::load_f32(xr + c));
+      if (rr != nullptr) s64 += static_cast<double>(detail::load_f32(rr + c));
+      if (a.w_dtype == XDT_F16) return s64 * static_cast<double>(detail::load_f32(static_cast<const __half*>(a.weight) + c));
+      if (a.w_dtype == XDT_BF16) return s64 * static_cast<double>(detail::load_f32(static_cast<const __nv_bfloat16*>(a.weight) + c));
+      return s64 * static_cast<double>(detail::load_f32(static_cast<const float*>(a.weight) + c));
+    };
+    const bool decide = row_ok && good && amax > 1e-5f;
+#pragma unroll
+    for (int m = 0; m < MW; ++m)
+      for (uint32_t left = decide ? largest[m] : 0u; left != 0; left &= left - 1) {
+        const int k = 32 * m + __ffs(left) - 1, c = at(k >> 3, k & 7);
+        if (c < a.D)  // positive 64-bit floats order as integers
+          atomicMax(&top64[sub], static_cast<unsigned long long>(__double_as_longlong(fabs(product64(c)))));
+      }
+    __syncthreads();
+    const double den = __longlong_as_double(static_cast<long long>(top64[sub])) * static_cast<double>(a.clip);
+#pragma unroll
+    for (int m = 0; m < MW; ++m)
+      for (uint32_t left = decide ? near[m] : 0u; left != 0; left &= left - 1) {
+        const int k = 32 * m + __ffs(left) - 1, c = at(k >> 3, k & 7);
+        if (c >= a.D) continue;
+        const double num = product64(c) * 448.0;
+        if (fabs(num) >= 0.015625 * den && fabs(num) < 448.0 * den)  // from 2^-6 on steps are relative: e4m3's normal range
+          q[c] = static_cast<uint8_t>(detail::code_e4m3x2(detail::nearest_e4m3(num, den), 0.0f));
+      }
   }
 }
 
 constexpr int kRmsNormMaxD = 16384;  // a row stays in the registers of 256 threads
 
-template <typename T, bool VEC>
-inline cudaError_t launch_rms_norm_quant(const RmsNormArgs& a, cudaStream_t stream) {
+template <typename T, bool VEC, bool E4M3>
+inline cudaError_t launch_rms_norm_quant_as(const RmsNormArgs& a, cudaStream_t stream) {
 #define B200W4A4_RMS_LAUNCH(TPR, NCH)                                                             \
   do {                                                                                             \
     constexpr int ROWS = 256 / (TPR);                                                              \
     const unsigned grid = static_cast<unsigned>((static_cast<long long>(a.M) + ROWS - 1) / ROWS);  \
-    rms_norm_quant_kernel<T, TPR, NCH, VEC><<<grid, 256, 0, stream>>>(a);                          \
+    rms_norm_quant_kernel<T, TPR, NCH, VEC, E4M3><<<grid, 256, 0, stream>>>(a);                          \
   } while (0)
   const int chunks = (a.D + 7) / 8;
   if (chunks <= 32) B200W4A4_RMS_LAUNCH(32, 1);
   else if (chunks <= 32 * 3) B200W4A4_RMS_LAUNCH(32, 3);
   else if (chunks <= 64 * 3) B200W4A4_RMS_LAUNCH(64, 3);
   else if (chunks <= 128 * 3) B200W4A4_RMS_LAUNCH(128, 3);
+  else if (chunks <= 128 * 5) B200W4A4_RMS_LAUNCH(128, 5);
   else if (chunks <= 256 * 3) B200W4A4_RMS_LAUNCH(256, 3);
   else if (chunks <= 256 * 5) B200W4A4_RMS_LAUNCH(256, 5);
   else B200W4A4_RMS_LAUNCH(256, 8);
 #undef B200W4A4_RMS_LAUNCH
   return cudaGetLastError();
+}
+
+template <typename T, bool VEC>
+inline cudaError_t launch_rms_norm_quant(const RmsNormArgs& a, cudaStream_t stream) {
+  return a.format == CODES_E4M3 ? launch_rms_norm_quant_as<T, VEC, true>(a, stream)
+                                : launch_rms_norm_quant_as<T, VEC, false>(a, stream);
 }
 
 }  // namespace b200w4a4

@@ -25,8 +25,8 @@ extern "C" {
  *   s = x + residual;  y = s * rsqrt(mean(s^2) + eps) * weight;  codes, scale of y (max|y| >= 1e-5)
  * x, residual [M, D] of x_dtype (F16, BF16, F32), row pitches x_ld / residual_ld; weight [D] of
  * w_dtype; codes [M, D] bytes; scale fp32 [M]; residual_out [M, D] of x_dtype = s rounded once.
- * residual and residual_out are both given or both NULL; residual_out may be x or residual itself
- * when that is contiguous.  The arithmetic is fp32 and reads s before its rounding.  1 <= D <= 16384.
+ * residual and residual_out are both given or both NULL.  The arithmetic is fp32 and reads s before its
+ * rounding; e4m3 codes are decided in 64 bits where fp32 cannot tell two neighbours apart.  1 <= D <= 16384.
  * int8 codes and scales are what b200w4a4_gemm and b200w4a4_linear_w4_group take.
  * A row that is not finite gets scale NaN and codes 0. */
 int b200w4a4_rms_norm_quant(const void* x, int x_dtype, long long x_ld, const void* residual,

@@ -38,7 +38,7 @@ def _rms(lib, **over):
     (dict(dt=3), -1), (dict(wdt=-1), -1), (dict(fmt=2), -1), (dict(r=P), -1), (dict(ro=P), -1), (dict(clip=0.0), -1),
     (dict(clip=float("nan")), -1), (dict(eps=-1.0), -1), (dict(m=-1), -2), (dict(d=0), -2), (dict(d=16385, ld=16385), -2),
     (dict(x=None), -1), (dict(w=None), -1), (dict(codes=None), -1), (dict(scale=None), -1), (dict(ld=63), -2),
-    (dict(r=P, ro=P, rld=10), -2), (dict(x=P + 1), -3), (dict(scale=P + 2), -3), (dict(m=0, x=None), 0),
+    (dict(r=P, ro=2 * P, rld=10), -2), (dict(r=P, ro=P), -1), (dict(r=2 * P, ro=P), -1), (dict(x=P + 1), -3), (dict(scale=P + 2), -3), (dict(m=0, x=None), 0),
 ])
 def test_rms_norm_quant_refusals(lib, over, code):
     assert _rms(lib, **over) == code

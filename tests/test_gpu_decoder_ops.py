@@ -103,6 +103,30 @@ def test_rms_norm_quant_small_zero_and_not_finite_rows():
     assert bool(torch.isnan(rms_norm_quant(x[:1], w)[1]).all())
 
 
+@pytest.mark.parametrize("dtype, d, clip", [(F32, 1536, 1.0), (BF, 5120, 1.0), (FP, 777, 0.9), (F32, 96, 1.0)])
+def test_rms_norm_quant_e4m3_codes_are_the_exact_ones(dtype, d, clip):
+    """Millions of values, none on the wrong side of a midpoint: the definition in 64 bits, rounded to the nearest e4m3
+    value with ties to even by a search over all of them."""
+    from dsaquant_b200.kernels.rms_norm import rms_norm_quant
+
+    g = _gen(41 + d)
+    m = 3_000_000 // d
+    x, r = _randn(g, m, d, dtype=dtype), _randn(g, m, d, dtype=dtype)
+    w = (1 + 0.1 * _randn(g, d)).to(dtype)
+    codes, scale, _ = rms_norm_quant(x, w, residual=r, out_dtype=torch.float8_e4m3fn, clip_ratio=clip)
+    y = (x.double() + r.double()) * w.double()                       # the rsqrt cancels in y / max|y|
+    t = (y * 448 / (y.abs().amax(-1, keepdim=True) * clip)).clamp(-448, 448)
+    table = torch.arange(127, device="cuda", dtype=torch.uint8).view(torch.float8_e4m3fn).double()   # 0 .. 448
+    mid = (table[1:] + table[:-1]) / 2
+    low = torch.searchsorted(mid, t.abs())                           # mid[low - 1] < |t| <= mid[low]
+    tie = (low < 126) & (t.abs() == mid[low.clamp(max=125)]) & (low % 2 == 1)
+    want = torch.where(t < 0, -1.0, 1.0) * table[low + tie.long()]
+    normal = t.abs() >= 2.0 ** -6
+    assert torch.equal(codes.double()[normal], want[normal])
+    # below the normal range the steps are absolute (2^-9) and an fp32 quotient is off by 2^-6 * 8 * 2^-24 at most
+    _within(codes.double()[~normal], t[~normal], 2.0 ** -10 + 2.0 ** -27)
+
+
 def test_rms_norm_quant_refusals_and_empty():
     from dsaquant_b200.kernels.rms_norm import rms_norm_quant
 
