@@ -101,7 +101,7 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[WORDS
 }  // namespace detail
 
 constexpr int kW4Warps = 8;
-constexpr int kW4WarpsPerSm = 48;  // at most so many warps an SM when K is split
+constexpr int kW4WarpsPerSm = 64;  // at most so many warps an SM when K is split
 // GB: codes that are sure to share a scale (32, 64 or 128; a divisor of the group).  A superblock is
 // 128 codes of a row; lane (g, t) multiplies the run of GB / 4 codes at t * GB / 4 of each of its 128 / GB
 // parts, for rows g and g + 8 of each of the RT row tiles.  NT: tiles of 8 tokens.
