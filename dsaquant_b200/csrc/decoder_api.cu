@@ -248,7 +248,11 @@ int b200w4a4_window_attention(const void* q, long long q_b, long long q_tok, lon
     a.part_lse = a.part_o + rows * head_dim;
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (a.Lq >= kAttnTcMinQueries && a.Lk > 0) {
+  // tensor maps take no pitch of 0 (heads or sequences that share memory) and none of 2^40 bytes
+  const int extents[9] = {B, Lq, q_heads, B, Lk, k_heads, B, Lk, k_heads};
+  bool mapped = true;
+  for (int i = 0; i < 9; ++i) mapped = mapped && (extents[i] <= 1 || (pitches[i] > 0 && pitches[i] < (1LL << 39)));
+  if (a.Lq >= kAttnTcMinQueries && a.Lk > 0 && mapped) {
     if (dtype == B200W4A4_F16)
       return head_dim == 64 ? launch_window_attn_tc<__half, 64>(a, dev, s) : launch_window_attn_tc<__half, 128>(a, dev, s);
     return head_dim == 64 ? launch_window_attn_tc<__nv_bfloat16, 64>(a, dev, s) : launch_window_attn_tc<__nv_bfloat16, 128>(a, dev, s);

@@ -117,7 +117,8 @@ __device__ __forceinline__ int swz(int r, int c) {
 
 }  // namespace attn
 
-// mma.sync form: four warps of 16 rows each, key tiles of 64 in two cp.async stages.
+// Short chunks (more rows than the single-token kernel takes, fewer than 128 queries), and prompts whose pitches no
+// tensor map can express: mma.sync, four warps of 16 rows each, key tiles of 64 in two cp.async stages.
 constexpr int kAttnRows = 64, kAttnBN = 64;
 
 template <typename T, int HD>

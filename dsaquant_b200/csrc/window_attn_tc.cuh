@@ -413,7 +413,8 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         const uint64_t sc2 = pair(sc, sc), neg2 = pair(neg, neg);
         uint64_t both = pair(0.0f, 0.0f);
         // Exponentials run LAG pairs ahead of their sums and conversions: a warp that asks for a result at once
-        // waits out the special-function unit's latency at every pair.
+        // waits out the special-function unit's latency at every pair.  (A quarter of them as a polynomial on the FMA pipe,
+        // made safe for masked, infinite and NaN scores, took 890 us instead of 850 at 12 heads x 32760.)
         constexpr int LAG = 4;
         float e[32];
         uint32_t w[16];

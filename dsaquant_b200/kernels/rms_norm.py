@@ -9,7 +9,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _lib
-from .vdm_w4a4 import _DTYPE_CODE, _DeviceGuard, _empty, _load_ext, _require_cuda, _stream_ptr
+from .vdm_w4a4 import _DTYPE_CODE, _empty, _load_ext, _require_cuda, _run, _stream_ptr
 
 _FORMATS = {torch.int8: 0, torch.float8_e4m3fn: 1}
 MAX_WIDTH = 16384
@@ -40,7 +40,8 @@ def rms_norm_quant(
         codes = clamp(rint(y / scale), -128, 127)         or y / scale rounded to e4m3, saturating
 
     Everything is fp32 and reads s before its rounding.  D is at most 16384.  Rows may be strided (views of a
-    wider tensor are read in place).  A row that holds an infinity or a NaN has scale NaN and codes 0."""
+    wider tensor are read in place).  A row whose sum of squares is not finite in fp32 (it
+    holds an infinity, a NaN, or values near 1e19) has scale NaN and codes 0.  Forward only, as every operator here."""
     lib = _load_ext()
     _require_cuda(x, "x")
     if x.dtype not in _DTYPE_CODE or weight.dtype not in _DTYPE_CODE:
@@ -63,15 +64,16 @@ def rms_norm_quant(
         stream_out = _empty(x.shape, x.dtype, dev)
     x2 = _rows(x, d)
     m = x2.shape[0]
+    if m >= 1 << 31:
+        raise ValueError("x must have fewer than 2^31 rows")
     w = weight if weight.is_contiguous() else weight.contiguous()
     codes = _empty(x.shape, out_dtype, dev)
     scale = _empty(x.shape[:-1], torch.float32, dev)
     if m > 0:
-        with _DeviceGuard(dev):
-            rc = lib.b200w4a4_rms_norm_quant(
-                x2.data_ptr(), _DTYPE_CODE[x.dtype], x2.stride(0) if m > 1 else d, r2.data_ptr() if r2 is not None else None,
-                r2.stride(0) if r2 is not None and m > 1 else d, w.data_ptr(), _DTYPE_CODE[w.dtype], float(eps),
-                codes.data_ptr(), _FORMATS[out_dtype], scale.data_ptr(),
-                stream_out.data_ptr() if stream_out is not None else None, m, d, float(clip_ratio), _stream_ptr(dev))
+        rc = _run(
+            dev, lib.b200w4a4_rms_norm_quant, x2.data_ptr(), _DTYPE_CODE[x.dtype], x2.stride(0) if m > 1 else d,
+            r2.data_ptr() if r2 is not None else None, r2.stride(0) if r2 is not None and m > 1 else d, w.data_ptr(),
+            _DTYPE_CODE[w.dtype], float(eps), codes.data_ptr(), _FORMATS[out_dtype], scale.data_ptr(),
+            stream_out.data_ptr() if stream_out is not None else None, m, d, float(clip_ratio), _stream_ptr(dev))
         _lib.check(rc, "rms_norm_quant")
     return (codes, scale) if residual is None else (codes, scale, stream_out)

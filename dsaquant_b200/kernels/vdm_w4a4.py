@@ -219,6 +219,17 @@ class _DeviceGuard:
         return False
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _run(device: torch.device, fn, *args) -> int:
+    """fn(*args) with `device` current; without the guard's object (0.6 us) where it is already."""
+    if _current_device() == device.index:
+        return fn(*args)
+    with _DeviceGuard(device):
+        return fn(*args)
+
+
 # --------------------------------------------------------------------------- weight side
 def pack_weight_with_scale(weight: torch.Tensor, channel_scale: torch.Tensor):
     """fp weight [N,K] + caller-provided per-channel scale -> the three vdm_w4a4_packed_v1

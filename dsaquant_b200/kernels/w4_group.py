@@ -12,9 +12,10 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _lib
-from .vdm_w4a4 import _DTYPE_CODE, _DeviceGuard, _empty, _load_ext, _require_cuda, _stream_ptr
+from .vdm_w4a4 import _DTYPE_CODE, _empty, _load_ext, _require_cuda, _run, _stream_ptr
 
 _X_CODE = {torch.float16: 0, torch.bfloat16: 1, torch.int8: 3}
+MAX_TOKENS = 65535 * 8
 _OUT_CODE = {torch.float16: 0, torch.bfloat16: 1}
 
 
@@ -31,9 +32,8 @@ def quantize_weight_grouped(weight: torch.Tensor, group_size: int = 128) -> Tupl
     w = weight.detach().contiguous()
     packed = torch.empty((n, k // 2), dtype=torch.uint8, device=w.device)
     scales = torch.empty((n, k // group_size), dtype=torch.float16, device=w.device)
-    with _DeviceGuard(w.device):
-        rc = lib.b200w4a4_quantize_weight_grouped(w.data_ptr(), _DTYPE_CODE[w.dtype], packed.data_ptr(), scales.data_ptr(),
-                                                  n, k, group_size, _stream_ptr(w.device))
+    rc = _run(w.device, lib.b200w4a4_quantize_weight_grouped, w.data_ptr(), _DTYPE_CODE[w.dtype], packed.data_ptr(),
+              scales.data_ptr(), n, k, group_size, _stream_ptr(w.device))
     _lib.check(rc, "quantize_weight_grouped")
     return packed, scales
 
@@ -75,6 +75,8 @@ def linear_w4_group(
     if not x2.is_contiguous() or x2.data_ptr() % 16:
         x2 = x2.clone(memory_format=torch.contiguous_format)
     m = x2.shape[0]
+    if m > MAX_TOKENS:
+        raise ValueError(f"at most {MAX_TOKENS} tokens a call")
     if not packed.is_contiguous() or packed.data_ptr() % 16 or not scales.is_contiguous():
         raise ValueError("packed (16-byte aligned) and scales must be contiguous")
     if (act_scale is not None) != (x.dtype == torch.int8):
@@ -90,10 +92,10 @@ def linear_w4_group(
             bias = bias.detach().to(out_dtype).contiguous()
     out = _empty((*x.shape[:-1], n), out_dtype, dev)
     if m > 0:
-        with _DeviceGuard(dev):
-            rc = lib.b200w4a4_linear_w4_group(
-                x2.data_ptr(), _X_CODE[x.dtype], act_scale.data_ptr() if act_scale is not None else None, packed.data_ptr(),
-                scales.data_ptr(), bias.data_ptr() if bias is not None else None, out.data_ptr(), _OUT_CODE[out_dtype], m, n,
-                k, k // groups, _stream_ptr(dev))
+        rc = _run(
+            dev, lib.b200w4a4_linear_w4_group, x2.data_ptr(), _X_CODE[x.dtype],
+            act_scale.data_ptr() if act_scale is not None else None, packed.data_ptr(), scales.data_ptr(),
+            bias.data_ptr() if bias is not None else None, out.data_ptr(), _OUT_CODE[out_dtype], m, n, k, k // groups,
+            _stream_ptr(dev))
         _lib.check(rc, "linear_w4_group")
     return out

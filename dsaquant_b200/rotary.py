@@ -11,7 +11,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .kernels.vdm_w4a4 import _DTYPE_CODE, _DeviceGuard, _empty, _load_ext, _require_cuda, _stream_ptr
+from .kernels.vdm_w4a4 import _DTYPE_CODE, _empty, _load_ext, _require_cuda, _run, _stream_ptr
 
 SCALINGS = ("none", "linear", "ntk", "yarn")
 
@@ -62,14 +62,6 @@ def rotary_table(
     return (torch.stack([angle.cos(), angle.sin()], -1) * amplitude).float()
 
 
-def _check_rows(x: torch.Tensor, name: str, like: Optional[torch.Tensor]) -> None:
-    if x.dim() != 3 or (x.shape[2] > 1 and x.stride(2) != 1):
-        raise ValueError(f"{name} must be [T, heads, head_dim] with unit stride in the head")
-    if like is not None and (x.shape[0] != like.shape[0] or x.shape[2] != like.shape[2] or x.dtype != like.dtype
-                             or x.device != like.device):
-        raise ValueError(f"{name} must match q in tokens, head_dim, dtype and device")
-
-
 def apply_rotary(
     q: torch.Tensor,
     k: Optional[torch.Tensor],
@@ -90,12 +82,19 @@ def apply_rotary(
     _require_cuda(q, "q")
     if q.dtype not in _DTYPE_CODE:
         raise RuntimeError("apply_rotary takes float16, bfloat16 or float32")
-    _check_rows(q, "q", None)
-    if k is not None:
-        _check_rows(k, "k", q)
-    dev = q.device
+    if q.dim() != 3 or (k is not None and k.dim() != 3):
+        raise ValueError("q and k must be [T, heads, head_dim]")
+    dev, dtype = q.device, q.dtype
     t, hq, hd = q.shape
-    hk = k.shape[1] if k is not None else 0
+    qs = q.stride()
+    hk, ks, kos, k_ptr, ko_ptr = 0, (0, 0, 1), (0, 0), None, None
+    if k is not None:
+        tk, hk, hdk = k.shape
+        ks, k_ptr = k.stride(), k.data_ptr()
+        if tk != t or hdk != hd or k.dtype != dtype or k.device != dev:
+            raise ValueError("k must match q in tokens, head_dim, dtype and device")
+    if hd > 1 and (qs[2] != 1 or ks[2] != 1):
+        raise ValueError("q and k must have unit stride in the head")
     if cos_sin.dim() != 3 or cos_sin.shape[2] != 2 or cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous():
         raise ValueError("cos_sin must be a contiguous float32 [positions, rotary_dim / 2, 2] table")
     rd = 2 * cos_sin.shape[1]
@@ -107,20 +106,19 @@ def apply_rotary(
         raise ValueError("q, cos_sin and positions must be on one device")
     if hq < 1 or (k is not None and hk < 1):
         raise ValueError("q and k must have heads")
-    if inplace:
-        q_out, k_out = q, k
-    else:
-        q_out = _empty((t, hq, hd), q.dtype, dev)
-        k_out = _empty((t, hk, hd), q.dtype, dev) if k is not None else None
+    if inplace and ((t > 1 and not (qs[0] and (k is None or ks[0]))) or (hq > 1 and not qs[1]) or (hk > 1 and not ks[1])):
+        raise ValueError("inplace needs tensors whose tokens and heads do not share memory")
+    q_out, k_out = (q, k) if inplace else (_empty((t, hq, hd), dtype, dev), None)
+    if k is not None:
+        if not inplace:
+            k_out = _empty((t, hk, hd), dtype, dev)
+        kos, ko_ptr = k_out.stride(), k_out.data_ptr()
     if t > 0:
         pos = positions if positions.is_contiguous() else positions.contiguous()
-        qs, qos = q.stride(), q_out.stride()
-        ks, kos = (k.stride(), k_out.stride()) if k is not None else ((0, 0), (0, 0))
-        with _DeviceGuard(dev):
-            rc = lib.b200w4a4_rotary(
-                q.data_ptr(), qs[0], qs[1], q_out.data_ptr(), qos[0], qos[1], hq, k.data_ptr() if k is not None else None,
-                ks[0], ks[1], k_out.data_ptr() if k is not None else None, kos[0], kos[1], hk, _DTYPE_CODE[q.dtype],
-                cos_sin.data_ptr(), cos_sin.shape[0], pos.data_ptr(), 1 if pos.dtype == torch.int64 else 0, t, hd, rd,
-                1 if interleaved else 0, 1 if inverse else 0, _stream_ptr(dev))
+        qos = q_out.stride()
+        rc = _run(
+            dev, lib.b200w4a4_rotary, q.data_ptr(), qs[0], qs[1], q_out.data_ptr(), qos[0], qos[1], hq, k_ptr, ks[0], ks[1],
+            ko_ptr, kos[0], kos[1], hk, _DTYPE_CODE[dtype], cos_sin.data_ptr(), cos_sin.shape[0], pos.data_ptr(),
+            1 if pos.dtype == torch.int64 else 0, t, hd, rd, 1 if interleaved else 0, 1 if inverse else 0, _stream_ptr(dev))
         _lib.check(rc, "rotary")
     return q_out, k_out

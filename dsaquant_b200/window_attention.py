@@ -7,7 +7,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from . import _lib
-from .kernels.vdm_w4a4 import _DeviceGuard, _empty, _load_ext, _require_cuda, _stream_ptr
+from .kernels.vdm_w4a4 import _empty, _load_ext, _require_cuda, _run, _stream_ptr
 
 _CODE = {torch.float16: 0, torch.bfloat16: 1}
 
@@ -59,6 +59,8 @@ def window_attention(
         raise ValueError("k and v must have q's batch and head_dim (64 or 128)")
     if hk < 1 or hq < 1 or hq % hk or hq // hk > 64:
         raise ValueError("q_heads must be a multiple (at most 64 times) of k_heads")
+    if max(b, lq, lk, hq) >= 1 << 31:
+        raise ValueError("sizes must be below 2^31")
     dev = q.device
     if k.dtype != q.dtype or v.dtype != q.dtype or k.device != dev or v.device != dev:
         raise ValueError("q, k and v must have one dtype and device")
@@ -77,12 +79,12 @@ def window_attention(
     if out.numel() > 0:
         (q, qs), (k, ks), (v, vs) = _readable(q), _readable(k), _readable(v)
         window, sinks = min(window, max(lk, 1)), min(sinks, lk)
-        with _DeviceGuard(dev):
-            need = lib.b200w4a4_window_attention_workspace_bytes(b, lq, lk, hq, hk, hd, window, sinks)
-            ws = _empty((need,), torch.uint8, dev) if need else None
-            rc = lib.b200w4a4_window_attention(
-                q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs, kv_lens.data_ptr() if kv_lens is not None else None,
-                out.data_ptr(), lse.data_ptr() if lse is not None else None, _CODE[q.dtype], b, lq, lk, hq, hk, hd, window,
-                sinks, scale, ws.data_ptr() if ws is not None else None, need, _stream_ptr(dev))
+        need = _run(dev, lib.b200w4a4_window_attention_workspace_bytes, b, lq, lk, hq, hk, hd, window, sinks)
+        ws = _empty((need,), torch.uint8, dev) if need else None
+        rc = _run(
+            dev, lib.b200w4a4_window_attention, q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs,
+            kv_lens.data_ptr() if kv_lens is not None else None, out.data_ptr(), lse.data_ptr() if lse is not None else None,
+            _CODE[q.dtype], b, lq, lk, hq, hk, hd, window, sinks, scale, ws.data_ptr() if ws is not None else None, need,
+            _stream_ptr(dev))
         _lib.check(rc, "window_attention")
     return (out, lse) if return_lse else out

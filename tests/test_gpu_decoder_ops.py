@@ -385,7 +385,9 @@ def test_apply_rotary_round_trip_gradient_and_refusals():
                 lambda: apply_rotary(x, None, rotary_table(4, 34, device="cuda"), pos),
                 lambda: apply_rotary(x.transpose(1, 2), None, table, pos), lambda: apply_rotary(x, x.float(), table, pos),
                 lambda: apply_rotary(x, None, table, pos.float()), lambda: apply_rotary(x, None, table.cpu(), pos),
-                lambda: apply_rotary(x[:, :0], None, table, pos)):
+                lambda: apply_rotary(x[:, :0], None, table, pos),
+                lambda: apply_rotary(x[:, :1].expand(5, 3, 32), None, table, pos, inplace=True),
+                lambda: apply_rotary(x, x[:1].expand(5, 2, 32), table, pos, inplace=True)):
         with pytest.raises(ValueError):
             bad()
     assert apply_rotary(x[:0], None, table, pos[:0])[0].shape == (0, 2, 32)
@@ -480,6 +482,26 @@ def test_window_attention_large_scores_and_scale():
     _check_attention(q, k, v, 100, 4, scale=0.5)
 
 
+@pytest.mark.parametrize("lq, dtype, hd", [(1, BF, 128), (3, FP, 64), (60, BF, 64), (400, BF, 128), (400, FP, 64)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_window_attention_not_finite_scores_reach_the_rows_that_see_them(lq, dtype, hd, value):
+    from dsaquant_b200.window_attention import window_attention
+
+    lk, window, sinks = 400, 90, 2
+    g = _gen(25)
+    q, k, v = _qkv(g, 1, lq, lk, 2, 1, hd, dtype)
+    q[..., 0] = 1.0
+    clean, clean_lse = window_attention(q, k, v, window, sinks, return_lse=True)
+    for key in (3, 130, 131, 192, 255, 333, 398, 399):               # every kind of place in a key tile
+        bad = k.clone()
+        bad[0, key, 0, 0] = value
+        out, lse = window_attention(q, bad, v, window, sinks, return_lse=True)
+        at = lk - lq + torch.arange(lq, device="cuda")
+        sees = (at >= key) & (key > at - window)
+        assert torch.equal(out[0, ~sees], clean[0, ~sees]) and torch.equal(lse[0][:, ~sees], clean_lse[0][:, ~sees])
+        assert bool(torch.isnan(out[0, sees]).all()) and not bool(torch.isfinite(lse[0][:, sees]).any())
+
+
 def test_window_attention_strided_views_and_head_major_cache():
     from dsaquant_b200.window_attention import window_attention
 
@@ -494,6 +516,17 @@ def test_window_attention_strided_views_and_head_major_cache():
         odd = torch.empty(2 * 200 * 2 * 128 + 1, device="cuda", dtype=BF)[1:].view(2, 200, 2, 128)
         odd.copy_(k)                                                               # two bytes off: copied first
         assert torch.equal(want, window_attention(q, odd, v, 50, 4))
+
+
+def test_window_attention_shared_heads_and_sequences():
+    """Keys that several heads or sequences share by a pitch of 0."""
+    g = _gen(26)
+    for lq in (1, 40, 300):
+        q = _randn(g, 2, lq, 4, 64, dtype=BF)
+        k = _randn(g, 1, 300, 1, 64, dtype=BF).expand(2, 300, 4, 64)
+        _check_attention(q, k, k, 100, 3)
+        one = k[:, :, :1]                                             # the prompt all sequences share
+        _check_attention(q, one, one, 100, 3)
 
 
 def test_window_attention_wide_window_is_causal_and_merges():
