@@ -6,6 +6,10 @@
 // The row is loaded once and stays in registers as fp32 through both reductions (sum of squares,
 // abs-max), so what moves is x, the residual in and out, one byte a value and four a row.
 //
+// Measured at 32760 x 5120 bf16 with residual: int8 179 us (6.55 TB/s on 7 bytes a value, 1.01 of the copy rate), e4m3 232 us;
+// fp16 without residual 112 us (4.5 TB/s: bound by the instructions between load and store).  Rows whose length or address
+// allows no 128-bit access move one value an access: 20000 x 5121 with residual 445 us, four times the copy.
+//
 // e4m3 codes are those of the exact quotient: its midpoints are 2^-4 of a value apart, so among millions of values
 // some always lie within the fp32 roundings of one, and a code on the wrong side is a step of 6 %.  A value whose
 // quotient lies within 16 fp32 steps of a midpoint (one in 2^15) is read again and decided in 64 bits, against the
@@ -291,6 +295,8 @@ inline cudaError_t launch_rms_norm_quant_as(const RmsNormArgs& a, cudaStream_t s
     rms_norm_quant_kernel<T, TPR, NCH, VEC, E4M3><<<grid, 256, 0, stream>>>(a);                          \
   } while (0)
   const int chunks = (a.D + 7) / 8;
+  // Threads a row by its length; four blocks of 256 threads an SM while 40 values a thread allow it (32760 x 5120 fp16
+  // without residual: 112 us, 139 with 24 values and 256 threads a row).
   if (chunks <= 32) B200W4A4_RMS_LAUNCH(32, 1);
   else if (chunks <= 32 * 3) B200W4A4_RMS_LAUNCH(32, 3);
   else if (chunks <= 64 * 3) B200W4A4_RMS_LAUNCH(64, 3);

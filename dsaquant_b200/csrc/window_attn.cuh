@@ -298,6 +298,8 @@ __global__ void __launch_bounds__(128) window_attn_kernel(const WindowAttnArgs a
 // Single tokens: at most 16 rows a tile.  What bounds it is reading the keys and values once, so a CTA's four warps
 // each take 16 keys of every 64-key tile through a ring of their own (cp.async, kAttnDecodeStages deep, no barrier
 // between the warps), keep their own maximum, sum and output, and meet at the end in shared memory.
+// Measured, 16 sequences of 0 to 8192 keys, 40 query and 8 key heads of 128, window 4096: 42 us with the joining kernel
+// for 206 MB (4.9 TB/s, 0.76 of the copy rate); the 64-row form above took 67.5.
 constexpr int kAttnDecodeRows = 16, kAttnDecodeStages = 3;
 
 template <typename T, int HD>

@@ -76,7 +76,9 @@ size_t b200w4a4_window_attention_workspace_bytes(int B, int Lq, int Lk, int q_he
  * j > p - window or j < sinks.  out [B, Lq, q_heads, head_dim] contiguous; lse fp32 [B, q_heads, Lq] or
  * NULL (natural log; what b200w4a4_attn_merge takes).  A query that sees nothing: out 0, lse -inf.
  * Keys that no query can see may hold anything.  window >= 1, sinks >= 0, scale > 0.
- * workspace: of the size above, 16-byte aligned, not shared by calls that may overlap. */
+ * workspace: of the size above, 16-byte aligned, not shared by calls that may overlap.
+ * Calls with 128 queries or more wait on barriers inside the kernel, each for at most a second; one that runs out
+ * leaves 106 in the device status word (b200w4a4_last_device_status), and rows of out unwritten. */
 int b200w4a4_window_attention(const void* q, long long q_b, long long q_tok, long long q_head,
                               const void* k, long long k_b, long long k_tok, long long k_head,
                               const void* v, long long v_b, long long v_tok, long long v_head,
