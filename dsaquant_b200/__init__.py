@@ -5,6 +5,9 @@
     dsaquant_b200.checkpoints.packed_checkpoint <-> vdm_infer.checkpoints.packed_checkpoint
     dsaquant_b200.attention_qkv.get_qkv_projections <-> modules.attention._get_qkv_projections
 
+Decoder-layer operators beside it (no counterpart in the reference): kernels.rms_norm, kernels.w4_group, rotary,
+window_attention.
+
 `install_as_vdm_infer()` registers these modules under the reference's import paths so
 existing callers pick them up without edits.
 """
