@@ -699,3 +699,60 @@ def test_operators_on_another_stream():
             outs.append([window_attention(q, k, v, 2048, 4) for _ in range(5)])
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for group in outs for o in group)
+
+
+def test_prompts_on_two_streams_beside_the_gemm():
+    """Prompt attention and the tcgen05 GEMM both want all of an SM's tensor memory: calls that overlap on two streams
+    wait for one another and give what they give alone."""
+    from dsaquant_b200.kernels import vdm_w4a4 as vdm
+    from dsaquant_b200.window_attention import window_attention
+
+    g = _gen(34)
+    q, k, v = _qkv(g, 1, 700, 1500, 8, 2, 128, BF)
+    packed, sp, _ = vdm.quantize_weight_per_channel(_randn(g, 1536, 1536, dtype=FP) * 0.02)
+    codes = torch.randint(-8, 8, (3000, 1536), generator=g, device="cuda", dtype=torch.int8)
+    scale = torch.rand(3000, generator=g, device="cuda")
+    want, want_gemm = window_attention(q, k, v, 400, 4), vdm.linear_prequantized(codes, scale, packed, sp)
+    torch.cuda.synchronize()
+    side = [torch.cuda.Stream() for _ in range(3)]
+    outs, gemms = [], []
+    for _ in range(10):
+        for st in side[:2]:
+            with torch.cuda.stream(st):
+                outs.append(window_attention(q, k, v, 400, 4))
+        with torch.cuda.stream(side[2]):
+            gemms.append(vdm.linear_prequantized(codes, scale, packed, sp))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs) and all(torch.equal(o, want_gemm) for o in gemms)
+    assert vdm.last_device_status() == 0
+
+
+def test_prompt_layer_captures_and_replays():
+    """A chunk of a prompt as a CUDA graph: lengths and positions are data."""
+    g = _gen(35)
+    layer = _Layer(g)
+    b, t = 2, 130
+    x, s = _randn(g, b, t, 512, dtype=BF), _randn(g, b, t, 512, dtype=BF)
+    fill = [_randn(g, b, 400, 2, 128, dtype=BF) for _ in range(2)]
+    cache = [c.clone() for c in fill]
+    pos, lens = torch.arange(t, device="cuda"), torch.full((b,), t, dtype=torch.int32, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer(x, s, cache, pos, lens)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer(x, s, cache, pos, lens)
+    for start in (0, 7, 200):
+        x.copy_(_randn(g, b, t, 512, dtype=BF))
+        pos.copy_(torch.arange(start, start + t, device="cuda"))
+        lens.copy_(torch.tensor([start + t, max(start - 50, 0)], device="cuda"))   # the second sequence ends before its rows
+        for c, f in zip(cache, fill):
+            c.copy_(f)
+        graph.replay()
+        got = [o.clone() for o in out] + [c.clone() for c in cache]
+        for c, f in zip(cache, fill):
+            c.copy_(f)
+        want = list(layer(x, s, cache, pos, lens)) + cache
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
