@@ -509,13 +509,22 @@ __global__ void __launch_bounds__(128) window_attn_join_kernel(const WindowAttnA
   const float base = m == -INFINITY ? 0.0f : m;
   float total = 0.0f;
   float acc[HD / 32] = {};
-  for (int s = 0; s < a.splits; ++s) {
-    const float l = a.part_lse[s * rows + row];
-    if (l == -INFINITY) continue;  // a run without keys: its partial output is not read
-    const float w = exp2_fast(l - base);
-    total += w;
+  for (int s0 = 0; s0 < a.splits; s0 += 4) {  // four runs' loads at a time
+    float w[4], o[4][HD / 32];
 #pragma unroll
-    for (int i = 0; i < HD / 32; ++i) acc[i] = fmaf(w, a.part_o[(s * rows + row) * HD + lane + 32 * i], acc[i]);
+    for (int u = 0; u < 4; ++u) w[u] = s0 + u < a.splits ? a.part_lse[(s0 + u) * rows + row] : -INFINITY;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i)  // a run without keys: its partial output is not read
+        o[u][i] = w[u] == -INFINITY ? 0.0f : a.part_o[((s0 + u) * rows + row) * HD + lane + 32 * i];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      w[u] = exp2_fast(w[u] - base);
+      total += w[u];
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i) acc[i] = fmaf(w[u], o[u][i], acc[i]);
+    }
   }
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   const int qi = static_cast<int>(row % a.Lq);

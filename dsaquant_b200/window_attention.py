@@ -10,14 +10,16 @@ from . import _lib
 from .kernels.vdm_w4a4 import _empty, _load_ext, _require_cuda, _run, _stream_ptr
 
 _CODE = {torch.float16: 0, torch.bfloat16: 1}
+PROMPT_QUERIES = 128  # from here on a call takes the kernel for prompts, which needs no workspace
 
 
 def _readable(x: torch.Tensor) -> Tuple[torch.Tensor, Tuple[int, ...]]:
     """x itself and its pitches when the kernel can read it in place (unit stride in the head, 16-byte steps), else a
     copy's.  The pitch of a dimension of one is 0: it is never used."""
-    if x.data_ptr() % 16 or x.stride(3) != 1:
+    s0, s1, s2, s3 = x.stride()
+    if s3 != 1 or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
-    s0, s1, s2, _ = x.stride()
+        s0, s1, s2, _ = x.stride()
     if (s0 | s1 | s2) & 7:
         n0, n1, n2, _ = x.shape
         s0, s1, s2 = s0 if n0 > 1 else 0, s1 if n1 > 1 else 0, s2 if n2 > 1 else 0
@@ -79,7 +81,9 @@ def window_attention(
     if out.numel() > 0:
         (q, qs), (k, ks), (v, vs) = _readable(q), _readable(k), _readable(v)
         window, sinks = min(window, max(lk, 1)), min(sinks, lk)
-        need = _run(dev, lib.b200w4a4_window_attention_workspace_bytes, b, lq, lk, hq, hk, hd, window, sinks)
+        need = 0  # of workspace: only calls of fewer queries split the keys
+        if lq < PROMPT_QUERIES:
+            need = _run(dev, lib.b200w4a4_window_attention_workspace_bytes, b, lq, lk, hq, hk, hd, window, sinks)
         ws = _empty((need,), torch.uint8, dev) if need else None
         rc = _run(
             dev, lib.b200w4a4_window_attention, q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs,
