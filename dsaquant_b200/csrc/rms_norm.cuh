@@ -125,7 +125,12 @@ __global__ void __launch_bounds__(256, NCH <= 5 ? 4 : 2) rms_norm_quant_kernel(c
   const T* rr = static_cast<const T*>(a.residual);
   if (rr != nullptr) rr += (row_ok ? row : 0) * a.r_ld;
   T* ro = static_cast<T*>(a.residual_out) + row * a.D;
-  if (threadIdx.x < ROWS) top64[threadIdx.x] = 0ull;
+  // Cleared by the row's own first thread: the barriers of the row's reductions (for one warp a row, which reduces with
+  // shuffles alone, the barrier of that warp) stand between this and the row's maxima.
+  if constexpr (E4M3) {
+    if (t == 0) top64[sub] = 0ull;
+    if constexpr (TPR == 32) __syncwarp();
+  }
   auto at = [&](int i, int e) { return VEC ? 8 * (t + i * TPR) + e : (8 * i + e) * TPR + t; };
 
   float v[NCH][8];
