@@ -9,7 +9,10 @@
 // of the tile sees are two runs of key tiles - [0, first) for the sinks and [w0, w1] for the window - and only
 // those are visited; the mask is evaluated only in tiles that some row does not see entirely.
 // Keys that no row of the tile sees are read as zeros, so whatever lies there (freed or unwritten cache
-// lines, NaN among them) has no effect.
+// lines, NaN among them) has no effect.  A key that some rows of the tile see and others do not enters the second
+// product of all of them, of the others with weight 0 - and 0 * inf is NaN.  A row whose sum of weights is finite
+// and whose output is not is therefore computed again from its own keys alone (row_by_definition), at the end and by the
+// warp that has it: V that is finite costs one test a value, and nothing in the loops.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -115,6 +118,50 @@ __device__ __forceinline__ int swz(int r, int c) {
   return r * HD + ((c ^ (r & 7)) << 3);
 }
 
+// W columns from c0 on of the output of query qi, head qh, over the keys that the row sees in the key tiles
+// [first, last) of BN keys: sum_j exp2(q . k_j * scale * log2(e) - lse2) v_j in fp32, lse2 the row's log-sum-exp (in units of
+// log2, finite) over these keys.  All lanes of a warp take part: each scores one of 32 keys, then each adds up its columns.
+template <typename T, int HD, int W, int BN, typename Out>
+__device__ __noinline__ void row_by_definition(const WindowAttnArgs& a, const Span& sp, int b, int qi, int qh, int first,
+                                               int last, float lse2, int c0, Out* out) {
+  const int lane = threadIdx.x & 31;
+  int len = a.Lk;
+  if (a.kv_lens != nullptr) len = min(max(a.kv_lens[b], 0), a.Lk);
+  const int p = len - a.Lq + qi, hk = qh / a.G;
+  const T* q = static_cast<const T*>(a.q) + b * a.q_b + qi * a.q_t + qh * a.q_h;
+  const T* kb = static_cast<const T*>(a.k) + b * a.k_b + hk * a.k_h;
+  const T* vb = static_cast<const T*>(a.v) + b * a.v_b + hk * a.v_h + c0 + lane;
+  const float sc = a.scale * kLog2e;
+  float acc[W / 32] = {};
+  for (int n = first; n < last; ++n)
+    for (int half = 0; half < BN; half += 32) {
+      const int j0 = (n < sp.n_sink ? n : sp.w0 + n - sp.n_sink) * BN + half, j = j0 + lane;
+      const bool sees = j <= p && (j > p - a.window || j < a.sinks);
+      float w = 0.0f;
+      if (sees) {
+        const T* k = kb + j * a.k_t;
+        float s = 0.0f;
+        for (int c = 0; c < HD; c += 8) {
+          const uint4 x = __ldg(reinterpret_cast<const uint4*>(q + c)), y = __ldg(reinterpret_cast<const uint4*>(k + c));
+          const T* xt = reinterpret_cast<const T*>(&x);
+          const T* yt = reinterpret_cast<const T*>(&y);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) s = fmaf(static_cast<float>(xt[i]), static_cast<float>(yt[i]), s);
+        }
+        w = exp2_fast(fmaf(s, sc, -lse2));
+      }
+      for (unsigned left = __ballot_sync(0xffffffffu, sees); left != 0; left &= left - 1) {
+        const int l = __ffs(left) - 1;
+        const float wl = __shfl_sync(0xffffffffu, w, l);
+        const T* v = vb + (j0 + l) * a.v_t;
+#pragma unroll
+        for (int i = 0; i < W / 32; ++i) acc[i] = fmaf(wl, static_cast<float>(v[32 * i]), acc[i]);
+      }
+    }
+#pragma unroll
+  for (int i = 0; i < W / 32; ++i) out[lane + 32 * i] = static_cast<Out>(acc[i]);
+}
+
 }  // namespace attn
 
 // Short chunks (more rows than the single-token kernel takes, fewer than 128 queries), and prompts whose pitches no
@@ -122,7 +169,7 @@ __device__ __forceinline__ int swz(int r, int c) {
 constexpr int kAttnRows = 64, kAttnBN = 64;
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(128) window_attn_kernel(const WindowAttnArgs a) {
+__global__ void __launch_bounds__(128) window_attn_kernel(const __grid_constant__ WindowAttnArgs a) {
   using namespace attn;
   constexpr int BN = kAttnBN, KT = HD / 16;
   extern __shared__ __align__(128) uint8_t smem_raw[];
@@ -275,22 +322,45 @@ __global__ void __launch_bounds__(128) window_attn_kernel(const WindowAttnArgs a
   for (int i = 0; i < 2; ++i) {
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-    if (!row_ok[i]) continue;
     const float inv = l[i] > 0.0f ? 1.0f / l[i] : (l[i] == 0.0f ? 0.0f : l[i]);
     const float lse2 = l[i] == 0.0f ? -INFINITY : m[i] + log2f(l[i]);
     const long long head_row = (static_cast<long long>(b) * a.Hq + qh[i]) * a.Lq + qi[i];
-    if (a.splits > 1) {
-      const long long at = static_cast<long long>(split) * a.B * a.Hq * a.Lq + head_row;
+    const long long at = static_cast<long long>(split) * a.B * a.Hq * a.Lq + head_row;
+    T* out = static_cast<T*>(a.out) + ((static_cast<long long>(b) * a.Lq + qi[i]) * a.Hq + qh[i]) * HD;
+    float finite = 0.0f;  // NaN once a value is not
+#pragma unroll
+    for (int h = 0; h < HD / 8; ++h)
+#pragma unroll
+      for (int j = 2 * i; j < 2 * i + 2; ++j) {
+        finite = fmaf(o[h][j], 0.0f, finite);
+        o[h][j] = l[i] == 0.0f ? 0.0f : o[h][j] * inv;
+      }
+    if (row_ok[i] && a.splits > 1) {
       if (t == 0) a.part_lse[at] = lse2;
       float2* po = reinterpret_cast<float2*>(a.part_o + at * HD) + t;
 #pragma unroll
-      for (int h = 0; h < HD / 8; ++h) po[4 * h] = make_float2(o[h][2 * i] * inv, o[h][2 * i + 1] * inv);
-    } else {
+      for (int h = 0; h < HD / 8; ++h) po[4 * h] = make_float2(o[h][2 * i], o[h][2 * i + 1]);
+    } else if (row_ok[i]) {
       if (t == 0 && a.lse != nullptr) a.lse[head_row] = lse2 * kLn2;
-      T* out = static_cast<T*>(a.out) + ((static_cast<long long>(b) * a.Lq + qi[i]) * a.Hq + qh[i]) * HD + 2 * t;
 #pragma unroll
       for (int h = 0; h < HD / 8; ++h)
-        *reinterpret_cast<uint32_t*>(out + 8 * h) = pack2(o[h][2 * i] * inv, o[h][2 * i + 1] * inv, T());
+        *reinterpret_cast<uint32_t*>(out + 8 * h + 2 * t) = pack2(o[h][2 * i], o[h][2 * i + 1], T());
+    }
+    const bool again = row_ok[i] && !(finite == 0.0f) && l[i] > 0.0f && l[i] < INFINITY;
+    unsigned left = __ballot_sync(0xffffffffu, again);
+    while (left != 0) {
+      const int src = (__ffs(left) - 1) & ~3;  // the row's four lanes hold the same qi, qh and lse2
+      left &= ~(0xfu << src);
+      const int ri = __shfl_sync(0xffffffffu, qi[i], src), rh = __shfl_sync(0xffffffffu, qh[i], src);
+      const float rl = __shfl_sync(0xffffffffu, lse2, src);
+      const long long r = (static_cast<long long>(b) * a.Hq + rh) * a.Lq + ri;
+      __syncwarp();
+      if (a.splits > 1)
+        row_by_definition<T, HD, HD, BN>(a, sp, b, ri, rh, first, last, rl, 0,
+                                         a.part_o + (static_cast<long long>(split) * a.B * a.Hq * a.Lq + r) * HD);
+      else
+        row_by_definition<T, HD, HD, BN>(a, sp, b, ri, rh, first, last, rl, 0,
+                                         static_cast<T*>(a.out) + ((static_cast<long long>(b) * a.Lq + ri) * a.Hq + rh) * HD);
     }
   }
 }
@@ -303,7 +373,7 @@ __global__ void __launch_bounds__(128) window_attn_kernel(const WindowAttnArgs a
 constexpr int kAttnDecodeRows = 16, kAttnDecodeStages = 3;
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(128) window_attn_decode_kernel(const WindowAttnArgs a) {
+__global__ void __launch_bounds__(128) window_attn_decode_kernel(const __grid_constant__ WindowAttnArgs a) {
   using namespace attn;
   constexpr int BN = kAttnBN, WN = 16, KT = HD / 16, CH = HD / 8, D = kAttnDecodeStages;
   constexpr int TILE = WN * HD;  // values of a warp's K (or V) tile
@@ -444,7 +514,9 @@ __global__ void __launch_bounds__(128) window_attn_decode_kernel(const WindowAtt
   float* po = reinterpret_cast<float*>(smem_raw);
   float* pm = po + 4 * kAttnDecodeRows * OP;
   float* pl = pm + 4 * kAttnDecodeRows;
+  float* redo = pl + 4 * kAttnDecodeRows;  // a row's log-sum-exp where it is computed again, else NaN
   __syncthreads();
+  if (threadIdx.x < kAttnDecodeRows) redo[threadIdx.x] = __int_as_float(0x7fc00000);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
@@ -460,6 +532,7 @@ __global__ void __launch_bounds__(128) window_attn_decode_kernel(const WindowAtt
   }
   __syncthreads();
   constexpr int LANES = HD / 4;  // threads of a row, four values each
+  bool again = false;
   for (int r = threadIdx.x / LANES; r <= r1 - r0; r += 128 / LANES) {
     const int c = threadIdx.x % LANES * 4;
     float top = -INFINITY;
@@ -479,17 +552,40 @@ __global__ void __launch_bounds__(128) window_attn_decode_kernel(const WindowAtt
     }
     const float inv = total > 0.0f ? 1.0f / total : (total == 0.0f ? 0.0f : total);
     const float lse2 = total == 0.0f ? -INFINITY : base + log2f(total);
+    float finite = 0.0f;  // NaN once a value is not
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      finite = fmaf(acc[i], 0.0f, finite);
+      acc[i] = total == 0.0f ? 0.0f : acc[i] * inv;
+    }
+    if (!(finite == 0.0f) && total > 0.0f && total < INFINITY) {
+      redo[r] = lse2;  // every thread of the row that finds one writes the same
+      again = true;
+    }
     const int qi = (r0 + r) / a.G, qh = hk * a.G + (r0 + r) % a.G;
     const long long head_row = (static_cast<long long>(b) * a.Hq + qh) * a.Lq + qi;
     if (a.splits > 1) {
       const long long at = static_cast<long long>(split) * a.B * a.Hq * a.Lq + head_row;
       if (c == 0) a.part_lse[at] = lse2;
       if (lse2 != -INFINITY)
-        *reinterpret_cast<float4*>(a.part_o + at * HD + c) = make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+        *reinterpret_cast<float4*>(a.part_o + at * HD + c) = make_float4(acc[0], acc[1], acc[2], acc[3]);
     } else {
       if (c == 0 && a.lse != nullptr) a.lse[head_row] = lse2 * kLn2;
       T* out = static_cast<T*>(a.out) + ((static_cast<long long>(b) * a.Lq + qi) * a.Hq + qh) * HD + c;
-      *reinterpret_cast<uint2*>(out) = make_uint2(pack2(acc[0] * inv, acc[1] * inv, T()), pack2(acc[2] * inv, acc[3] * inv, T()));
+      *reinterpret_cast<uint2*>(out) = make_uint2(pack2(acc[0], acc[1], T()), pack2(acc[2], acc[3], T()));
+    }
+  }
+  if (__syncthreads_or(again)) {
+    for (int r = warp; r <= r1 - r0; r += 4) {
+      if (isnan(redo[r])) continue;
+      const int qi = (r0 + r) / a.G, qh = hk * a.G + (r0 + r) % a.G;
+      const long long head_row = (static_cast<long long>(b) * a.Hq + qh) * a.Lq + qi;
+      if (a.splits > 1)
+        row_by_definition<T, HD, HD, BN>(a, sp, b, qi, qh, first, last, redo[r], 0,
+                                         a.part_o + (static_cast<long long>(split) * a.B * a.Hq * a.Lq + head_row) * HD);
+      else
+        row_by_definition<T, HD, HD, BN>(a, sp, b, qi, qh, first, last, redo[r], 0,
+                                         static_cast<T*>(a.out) + ((static_cast<long long>(b) * a.Lq + qi) * a.Hq + qh) * HD);
     }
   }
 }
@@ -561,7 +657,7 @@ template <typename T, int HD>
 inline cudaError_t launch_window_attn(const WindowAttnArgs& a, cudaStream_t stream) {
   const long long rows = static_cast<long long>(a.Lq) * a.G;
   const bool decode = window_attn_decodes(rows);
-  constexpr int ring = 4 * kAttnDecodeStages * 2 * 16 * HD * 2, meet = 4 * kAttnDecodeRows * (HD + 8 + 2) * 4;
+  constexpr int ring = 4 * kAttnDecodeStages * 2 * 16 * HD * 2, meet = 4 * kAttnDecodeRows * (HD + 8 + 2) * 4 + 4 * kAttnDecodeRows;
   const int smem = decode ? (ring > meet ? ring : meet) : 4 * kAttnBN * HD * 2;
   const int per_tile = decode ? kAttnDecodeRows : kAttnRows;
   const auto kernel = decode ? window_attn_decode_kernel<T, HD> : window_attn_kernel<T, HD>;

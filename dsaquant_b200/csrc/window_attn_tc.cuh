@@ -23,7 +23,8 @@
 // it, and O is hardly ever rescaled.
 //
 // V rows of keys that no row of the CTA sees are overwritten with zeros in shared memory (by each tile's threads,
-// before they hand over P): 0 * garbage must not reach O.  Every wait is bounded.
+// before they hand over P): 0 * garbage must not reach O.  What a key that only some rows see holds is dealt with at the
+// end (row_by_definition).  Every wait is bounded.
 //
 // Measured, 12 heads of 128 x 32760 queries, window 4096, 64 first keys, bf16: 850 us, 0.786 TFLOP at 925 TFLOP/s, 0.56 of the
 // library product's burst rate (the mma.sync form: 2842 us).  Tensor pipe and special-function unit are each 46 % busy:
@@ -132,7 +133,7 @@ __device__ __forceinline__ bool tile_active(int p0, int p1, int j0, int window, 
 template <typename T, int HD>
 __global__ void __launch_bounds__(AttnTcCfg<HD>::THREADS, 1)
 window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                      const __grid_constant__ CUtensorMap tm_v, const AttnTcParams prm) {
+                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttnTcParams prm) {
   using namespace attn;
   using C = AttnTcCfg<HD>;
   const WindowAttnArgs& a = prm.a;
@@ -465,10 +466,14 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     }
     l = exchange(l, [](float u, float v) { return u + v; });
     const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+    const float lse2 = l == 0.0f ? -INFINITY : m + log2f(l);
     const bool ok = qi < a.Lq && alive;
-    if (h == 0 && ok && a.lse != nullptr)
-      a.lse[(static_cast<long long>(b) * a.Hq + hq) * a.Lq + qi] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
-    T* out = static_cast<T*>(a.out) + ((static_cast<long long>(b) * a.Lq + qi) * a.Hq + hq) * HD + h * (HD / 2);
+    if (h == 0 && ok && a.lse != nullptr) a.lse[(static_cast<long long>(b) * a.Hq + hq) * a.Lq + qi] = lse2 * kLn2;
+    auto out_of = [&](int query) {
+      return static_cast<T*>(a.out) + ((static_cast<long long>(b) * a.Lq + query) * a.Hq + hq) * HD + h * (HD / 2);
+    };
+    T* out = out_of(qi);
+    float finite = 0.0f;  // NaN once a value is not
 #pragma unroll 1
     for (int c = 0; c < HD / 64; ++c) {
       uint32_t o[32];
@@ -476,6 +481,12 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         ptx::tmem_ld_32x32(t_o + 32 * c, o);
         ptx::tmem_ld_wait_for(o);
       } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = 0u;
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) finite = fmaf(__uint_as_float(o[i]), 0.0f, finite);
+      if (l == 0.0f) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) o[i] = 0u;
       }
@@ -489,6 +500,14 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
           *reinterpret_cast<uint4*>(out + 32 * c + 8 * i) = make_uint4(v[0], v[1], v[2], v[3]);
         }
       }
+    }
+    unsigned left = __ballot_sync(0xffffffffu, ok && !(finite == 0.0f) && l > 0.0f && l < INFINITY);
+    __syncwarp();
+    for (; left != 0; left &= left - 1) {
+      const int src = __ffs(left) - 1;
+      const int query = i0 + x * C::BM + (warp & 3) * 32 + src;
+      row_by_definition<T, HD, HD / 2, C::BN>(a, sp, b, query, hq, 0, sp.n, __shfl_sync(0xffffffffu, lse2, src), h * (HD / 2),
+                                              out_of(query));
     }
   }
 

@@ -4,7 +4,7 @@ test_gpu_decoder_ops."""
 import pytest
 import torch
 
-from test_gpu_decoder_ops import BF, F32, FP, _gen, _randn
+from test_gpu_decoder_ops import BF, F32, FP, HALF_STEP, HALF_SUB, _attention64, _gen, _qkv, _randn, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +37,68 @@ def test_rms_norm_quant_e4m3_short_rows_share_a_block(d, dtype):
     t = y * 448 / y.abs().amax(-1, keepdim=True)
     normal = t.abs() >= 2.0 ** -6
     assert torch.equal(codes.double()[normal], _nearest_e4m3(t)[normal])
+
+
+# ------------------------------------------------------------------------------------------------ window_attention
+def _attention_bound(q, k, v, window, sinks, lens):
+    """The definition in 64 bits and how far a result may be off (the terms are explained at _check_attention)."""
+    lk, hd = k.shape[1], q.shape[3]
+    want, lse, spread, low, worst = _attention64(q, k, v, window, sinks, lens, hd ** -0.5)
+    ds = ((hd + 4) * 2.0 ** -23 * worst + 2.0 ** -21 * (1 + lk / 64 / 16)).transpose(1, 2)[..., None]
+    half, sub = HALF_STEP[q.dtype], HALF_SUB[q.dtype]
+    return want, half * want.abs() + sub + (half + 2 * ds + lk * 2.0 ** -23) * spread + sub * low
+
+
+@pytest.mark.parametrize("dtype, hd", [(BF, 128), (FP, 64)])
+@pytest.mark.parametrize("lq, hq, hk, lens, window, sinks", [
+    (3, 2, 2, (400, 1), 90, 2), (16, 4, 2, (400, 5), 5000, 0), (2, 8, 1, (1500, 700), 1000, 70), (60, 4, 2, (400, 30), 90, 2),
+    (127, 2, 1, (1500, 64), 5000, 0), (400, 2, 1, (400, 100), 90, 70), (300, 2, 2, (1500, 200), 700, 5), (200, 4, 1, (500, 199), 5000, 0)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_window_attention_not_finite_values_reach_only_the_rows_that_see_them(lq, hq, hk, lens, window, sinks, dtype, hd, value):
+    """A value of V that is not finite changes its own column of the rows that see its key, and nothing else: not the rows
+    before the key, not those past the window, not those that see nothing."""
+    from dsaquant_b200.window_attention import window_attention
+
+    g = _gen(61 + lq + hq)
+    lk = lens[0]
+    q, k, v = _qkv(g, 2, lq, lk, hq, hk, hd, dtype)
+    kv_lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    clean, clean_lse = window_attention(q, k, v, window, sinks, kv_lens=kv_lens, return_lse=True)
+    want, bound = _attention_bound(q, k, v, window, sinks, kv_lens)
+    for last in (0, 1, lq // 2, lq - 1):                              # keys that the query `last` and those behind it see
+        for column in (0, hd - 1, slice(None)):
+            bad = v.clone()
+            hit = torch.zeros(want.shape, dtype=torch.bool, device="cuda")
+            for i, n in enumerate(lens):
+                at = n - lq + torch.arange(lq, device="cuda")
+                key = max(n - lq + last, 0)
+                bad[i, key, hk - 1, column] = value
+                sees = (at >= key) & ((at < key + window) | (key < sinks))
+                rows = torch.zeros(lq, hq, hd, dtype=torch.bool, device="cuda")
+                rows[:, hq - hq // hk:, column] = True                # the heads that share the last key head
+                hit[i] = rows & sees[:, None, None]
+            out, lse = window_attention(q, k, bad, window, sinks, kv_lens=kv_lens, return_lse=True)
+            assert torch.equal(lse, clean_lse)
+            assert not bool(torch.isfinite(out[hit]).any())
+            _within(torch.where(hit, 0.0, out), torch.where(hit, 0.0, want), bound)
+            for i, n in enumerate(lens):
+                none = n - lq + torch.arange(lq, device="cuda") < 0
+                assert bool((out[i, none] == 0).all())
+            again = window_attention(q, k, bad, window, sinks, kv_lens=kv_lens)
+            assert torch.equal(out.view(torch.int16), again.view(torch.int16))
+    assert torch.equal(clean, window_attention(q, k, v, window, sinks, kv_lens=kv_lens))
+
+
+def test_window_attention_every_value_not_finite():
+    """A whole prompt of NaN is slow at worst: it ends, rows that see nothing are 0, all others NaN."""
+    from dsaquant_b200.kernels import vdm_w4a4 as vdm
+    from dsaquant_b200.window_attention import window_attention
+
+    g = _gen(62)
+    for lq in (4, 100, 1000):
+        q, k, v = _qkv(g, 2, lq, 1000, 4, 2, 128, BF)
+        lens = torch.tensor([1000, lq // 2], dtype=torch.int32, device="cuda")
+        out = window_attention(q, k, torch.full_like(v, float("nan")), 300, 4, kv_lens=lens)
+        assert bool(torch.isnan(out[0]).all()) and bool(torch.isnan(out[1, lq - lq // 2:]).all())
+        assert bool((out[1, :lq - lq // 2] == 0).all())
+    assert vdm.last_device_status() == 0
