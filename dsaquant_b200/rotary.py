@@ -62,6 +62,43 @@ def rotary_table(
     return (torch.stack([angle.cos(), angle.sin()], -1) * amplitude).float()
 
 
+def _distinct(x: torch.Tensor) -> bool:
+    """Whether no two values of x [T, heads, head_dim] share memory: each stride steps over everything below it.  (A layout
+    that interleaves its dimensions otherwise is counted as shared.)"""
+    span = 1
+    for stride, size in sorted((s, n) for s, n in zip(x.stride(), x.shape) if n > 1):
+        if stride < span:
+            return False
+        span = stride * (size - 1) + span
+    return True
+
+
+def _disjoint(q: torch.Tensor, k: torch.Tensor) -> bool:
+    """Whether q and k, [T, heads, head_dim] without shared values of their own, share no memory: one lies behind the other,
+    or in the gaps that the other's tokens or heads leave at the same stride (views of a fused projection)."""
+    apart = k.data_ptr() - q.data_ptr()
+    if apart < 0:
+        q, k, apart = k, q, -apart
+    apart, rest = divmod(apart, q.element_size())  # k starts so many values behind q
+    stride = [max(x.stride(i) if x.shape[i] > 1 else 0 for x in (q, k)) for i in range(3)]
+    dims = sorted((i for i in range(3) if stride[i]), key=lambda i: stride[i])
+
+    def reach(x: torch.Tensor) -> int:
+        return sum(x.stride(i) * (x.shape[i] - 1) for i in dims if x.shape[i] > 1) + 1
+
+    if apart >= reach(q):
+        return True
+    while dims and not rest:
+        step = dims.pop()  # the widest step: both lie within a stride of it, or are counted as shared
+        s = stride[step]
+        apart %= s
+        if any(x.shape[step] > 1 and x.stride(step) != s for x in (q, k)) or reach(q) > s or apart + reach(k) > s:
+            return False
+        if apart >= reach(q):
+            return True
+    return False
+
+
 def apply_rotary(
     q: torch.Tensor,
     k: Optional[torch.Tensor],
@@ -76,7 +113,8 @@ def apply_rotary(
     `positions` (int32 or int64 [T]) of cos_sin, a table as `rotary_table` makes it; its second dimension says how much
     of the head is rotated, the rest is copied.  Token and head strides are free.  interleaved: pairs (2i, 2i + 1)
     instead of (i, i + rotary_dim / 2).  inverse: rotates back (the transpose; also the gradient).
-    Returns new contiguous tensors, or with inplace the given ones, overwritten.
+    Returns new contiguous tensors, or with inplace the given ones, overwritten (q and k must not share memory then, nor
+    may tokens or heads of one of them).
     A token at a negative position (padding) is copied unchanged; one behind the table comes out as NaN."""
     lib = _load_ext()
     _require_cuda(q, "q")
@@ -106,8 +144,8 @@ def apply_rotary(
         raise ValueError("q, cos_sin and positions must be on one device")
     if hq < 1 or (k is not None and hk < 1):
         raise ValueError("q and k must have heads")
-    if inplace and ((t > 1 and not (qs[0] and (k is None or ks[0]))) or (hq > 1 and not qs[1]) or (hk > 1 and not ks[1])):
-        raise ValueError("inplace needs tensors whose tokens and heads do not share memory")
+    if inplace and t > 0 and not (_distinct(q) and (k is None or (_distinct(k) and _disjoint(q, k)))):
+        raise ValueError("inplace needs q and k whose tokens and heads share no memory, with one another either")
     q_out, k_out = (q, k) if inplace else (_empty((t, hq, hd), dtype, dev), None)
     if k is not None:
         if not inplace:

@@ -155,3 +155,45 @@ def test_rotary_tables_follow_their_formulas():
 def test_workspace_query_of_bad_or_empty_shapes_is_zero(lib):
     assert lib.b200w4a4_window_attention_workspace_bytes(0, 1, 4, 2, 1, 64, 4, 0) == 0
     assert lib.b200w4a4_window_attention_workspace_bytes(1, 1, 4, 3, 2, 64, 4, 0) == 0
+
+
+def test_shared_memory_of_q_and_k_is_found():
+    """`_distinct` and `_disjoint` against the addresses themselves: never true where two values share one, and true for the
+    views that a fused projection or a head-major cache gives."""
+    import random
+
+    from dsaquant_b200.rotary import _disjoint, _distinct
+
+    def addresses(x):
+        at = torch.arange(int(x.untyped_storage().nbytes()) // x.element_size())
+        return at.as_strided(x.shape, x.stride(), x.storage_offset()).flatten().tolist()
+
+    rng = random.Random(5)
+    flat = torch.zeros(4096)
+    said = [0, 0]
+    for _ in range(4000):
+        def some():
+            shape = [rng.choice([1, 2, 3]), rng.choice([1, 2, 3]), rng.choice([1, 2, 4])]
+            return shape, [rng.choice([0, 1, 2, 4, 8, 12, 16, 24]), rng.choice([0, 1, 4, 8, 12, 16]), 1], rng.randrange(40)
+        (n1, s1, o1), (n2, s2, o2) = some(), some()
+        if rng.random() < 0.6:
+            s2, n2 = s1, [n1[0], n2[1], n1[2]]
+        q, k = flat.as_strided(n1, s1, o1), flat.as_strided(n2, s2, o2)
+        a, b = addresses(q), addresses(k)
+        if _distinct(q):
+            assert len(set(a)) == len(a)
+        if _distinct(q) and _distinct(k):
+            said[_disjoint(q, k)] += 1
+            if _disjoint(q, k):
+                assert not set(a) & set(b) and _disjoint(k, q)
+    assert min(said) > 200
+    t, hq, hk, hd = 5, 6, 2, 8
+    for views in (lambda x: (x[:, :hq], x[:, hq:hq + hk]), lambda x: (x[:, hk:hk + hq], x[:, :hk])):
+        by_token = torch.zeros(t, hq + 2 * hk, hd)
+        by_head = torch.zeros(hq + 2 * hk, t, hd).transpose(0, 1)
+        for q, k in (views(by_token), views(by_head), views(by_token[2:3]), views(by_head[2:3])):
+            assert _distinct(q) and _distinct(k) and _disjoint(q, k)
+    each = torch.zeros(t, hq, 3, hd)                       # q, k and v of a head side by side
+    assert _disjoint(each[:, :, 0], each[:, :, 1]) and _disjoint(each[:, :, 2], each[:, :, 0])
+    assert not _disjoint(each[:, :, 0], each[:, :, 0]) and not _disjoint(by_token[:, :3], by_token[:, 2:4])
+    assert _disjoint(torch.zeros(t, hq, hd), torch.zeros(t, hk, hd))

@@ -102,3 +102,25 @@ def test_window_attention_every_value_not_finite():
         assert bool(torch.isnan(out[0]).all()) and bool(torch.isnan(out[1, lq - lq // 2:]).all())
         assert bool((out[1, :lq - lq // 2] == 0).all())
     assert vdm.last_device_status() == 0
+
+
+# ------------------------------------------------------------------------------------------------ apply_rotary
+def test_apply_rotary_inplace_refuses_shared_memory():
+    """q and k that overlap each other, or tokens that overlap, would be rotated twice; out of place they are read only."""
+    from dsaquant_b200.rotary import apply_rotary, rotary_table
+
+    g = _gen(71)
+    table, pos = rotary_table(64, 32, device="cuda"), torch.arange(5, device="cuda")
+    x = _randn(g, 5, 6, 32, dtype=FP)
+    sliding = _randn(g, 5 * 16 + 48, dtype=FP).as_strided((5, 2, 32), (16, 32, 1))
+    keep = x.clone()
+    for q, k in ((x, x), (x[:, :4], x[:, 3:]), (x[:, 2:], x[:, :3]), (x, x[:, 5:]), (sliding, None), (x, sliding)):
+        with pytest.raises(ValueError):
+            apply_rotary(q, k, table, pos, inplace=True)
+        rq, rk = apply_rotary(q, k, table, pos)
+        assert torch.equal(rq, apply_rotary(q.clone(), None, table, pos)[0])
+        assert k is None or torch.equal(rk, apply_rotary(k.clone(), None, table, pos)[0])
+    assert torch.equal(x, keep)
+    want = [apply_rotary(part.clone(), None, table, pos)[0] for part in (x[:, 2:], x[:, :2])]
+    got = apply_rotary(x[:, 2:], x[:, :2], table, pos, inplace=True)          # k in front of q
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(torch.cat([want[1], want[0]], 1), x)
