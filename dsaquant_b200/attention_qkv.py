@@ -26,18 +26,20 @@ def _cat_cached(attn, prefix: str, layers) -> None:
     concatenated tensors (same bytes, still saved per layer by a state dict), and the per-layer
     repacked weights, which the fused path never reads, are dropped from the repack table."""
     if getattr(attn, f"{prefix}_weight_packed", None) is None:
-        from .kernels.vdm_w4a4 import release_b200_weight
+        from .kernels.vdm_w4a4 import mark_gemm_layout, release_b200_weight
 
         packed = torch.cat([l.vdm_weight_packed for l in layers], dim=0).contiguous()
         scale = torch.cat([l.vdm_weight_scale_packed for l in layers], dim=0).contiguous()
         setattr(attn, f"{prefix}_weight_packed", packed)
         setattr(attn, f"{prefix}_weight_scale", scale)
+        mark_gemm_layout(packed, scale)
         row = 0
         for l in layers:
             n = l.vdm_weight_packed.shape[0]
             release_b200_weight(l.vdm_weight_packed)
             l._buffers["vdm_weight_packed"] = packed[row:row + n]
             l._buffers["vdm_weight_scale_packed"] = scale[row:row + n]
+            mark_gemm_layout(l.vdm_weight_packed, l.vdm_weight_scale_packed)
             row += n
     if not hasattr(attn, f"{prefix}_bias_half") or getattr(attn, f"{prefix}_bias_half") is None:
         n = layers[0].vdm_weight_packed.shape[0]

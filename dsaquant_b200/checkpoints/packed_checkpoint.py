@@ -23,6 +23,8 @@ from typing import Any, Dict, Iterable, List, Tuple
 import torch
 import torch.nn as nn
 
+from dsaquant_b200.kernels.vdm_w4a4 import mark_gemm_layout
+
 PACKED_CHECKPOINT_FORMAT = "vdm_w4a4_packed_v1"
 VDM_BUFFER_SUFFIXES = ("vdm_weight_packed", "vdm_weight_scale_packed", "vdm_weight_scale")
 _LEGACY_PACKED_CHECKPOINT_FORMAT = PACKED_CHECKPOINT_FORMAT.replace("vdm_", "vdm_diy_", 1)
@@ -79,6 +81,7 @@ def _switch_layer_to_packed(layer: nn.Module, buffers: Dict[str, torch.Tensor]) 
     """Attach the packed buffers and drop what they replace (fp weight, both fake quantisers)."""
     for name, tensor in buffers.items():
         _replace_buffer(layer, name, tensor)
+    mark_gemm_layout(layer.vdm_weight_packed, layer.vdm_weight_scale_packed)
     layer.use_vdm_kernel = True
     layer.use_kernel = layer.use_kernel_fused = False
     layer.set_quant_state(use_wq=True, use_aq=True)

@@ -231,6 +231,17 @@ def _run(device: torch.device, fn, *args) -> int:
 
 
 # --------------------------------------------------------------------------- weight side
+def mark_gemm_layout(*tensors: torch.Tensor) -> None:
+    """Notes on the tensors themselves that their values lie in an order of the GEMM (vdm_w4a4_packed_v1, or the repacked
+    form).  By type and shape such a weight cannot be told from a row-major one with scales for groups of 64."""
+    for t in tensors:
+        t._gemm_layout = True
+
+
+def in_gemm_layout(t: torch.Tensor) -> bool:
+    return getattr(t, "_gemm_layout", False) or getattr(t._base, "_gemm_layout", False)  # itself, or what it is a view of
+
+
 def pack_weight_with_scale(weight: torch.Tensor, channel_scale: torch.Tensor):
     """fp weight [N,K] + caller-provided per-channel scale -> the three vdm_w4a4_packed_v1
     buffers (qweight u8 [N,K/2], packed_scales f16 [N,K/64], channel_scales f16 [N])."""
@@ -263,6 +274,7 @@ def _pack(lib, weight_h: torch.Tensor, scale_h: Optional[torch.Tensor]):
             qweight.data_ptr(), packed_scales.data_ptr(), channel_scales.data_ptr(), n, k,
             _stream_ptr(dev))
     _lib.check(rc, "pack_weight")
+    mark_gemm_layout(qweight, packed_scales)
     return qweight, packed_scales, channel_scales
 
 
@@ -310,6 +322,7 @@ def prepare_b200_weight(qweight: torch.Tensor, wscales: torch.Tensor):
         rc = lib.b200w4a4_repack_weight(qw.data_ptr(), w_b200.data_ptr(), ws.data_ptr(),
                                         w_scale.data_ptr(), n, k, _stream_ptr(dev))
     _lib.check(rc, "repack_weight")
+    mark_gemm_layout(qweight, wscales, w_b200)
     _PREPARED[key] = (w_b200, w_scale)
     weakref.finalize(qweight, _PREPARED.pop, key, None)
     return w_b200, w_scale

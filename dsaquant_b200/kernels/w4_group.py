@@ -4,6 +4,10 @@
 A weight is two tensors, usable as they are (nothing is laid out or kept for it):
     packed  uint8 [N, K/2]        code 2b in the low and 2b + 1 in the high nibble of byte b, two's complement
     scales  float16 [N, K/group]  one for every `group` consecutive codes of a row (a multiple of 32)
+The weights of that GEMM (vdm_w4a4_packed_v1: the buffers of QuantLinear and of packed checkpoints) have the same types and,
+for groups of 64, the same shapes, but their codes and scales lie in the order of its tiles.  `regroup_packed_weight` turns one
+into the form used here, with the same codes and scales; the tensors that this package makes, loads or has used as
+such weights are refused (a copy that a program makes of one by hand is not known as one).
 """
 from __future__ import annotations
 
@@ -12,7 +16,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _lib
-from .vdm_w4a4 import _DTYPE_CODE, _empty, _load_ext, _require_cuda, _run, _stream_ptr
+from .vdm_w4a4 import _DTYPE_CODE, _empty, _load_ext, _require_cuda, _run, _stream_ptr, in_gemm_layout, unpack_codes
 
 _X_CODE = {torch.float16: 0, torch.bfloat16: 1, torch.int8: 3}
 MAX_TOKENS = 65535 * 8
@@ -38,6 +42,20 @@ def quantize_weight_grouped(weight: torch.Tensor, group_size: int = 128) -> Tupl
     return packed, scales
 
 
+def regroup_packed_weight(qweight: torch.Tensor, channel_scales: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """vdm_w4a4_packed_v1 codes [N, K/2] and their plain per-channel scales fp16 [N] (`vdm_weight_packed` and
+    `vdm_weight_scale` of a layer, the first and third result of `quantize_weight_per_channel`) -> (packed, scales [N, 1]): the
+    same weight with one group a row, for prompts through the GEMM and tokens through `linear_w4_group`."""
+    _require_cuda(qweight, "qweight")
+    n, k = qweight.shape[0], 2 * qweight.shape[1]
+    if qweight.dtype != torch.uint8 or qweight.dim() != 2 or n % 128 or k % 64 or n * k == 0:
+        raise ValueError("qweight must be uint8 [N, K/2] with N a multiple of 128 and K one of 64")
+    if channel_scales.dtype != torch.float16 or channel_scales.shape != (n,) or channel_scales.device != qweight.device:
+        raise ValueError("channel_scales must be float16 [N] on qweight's device")
+    codes = unpack_codes(qweight, n, k, 2).view(torch.uint8)
+    return codes[:, 0::2].bitwise_and(15) | codes[:, 1::2] << 4, channel_scales.detach().clone().unsqueeze(1)
+
+
 def linear_w4_group(
     x: torch.Tensor,
     packed: torch.Tensor,
@@ -58,6 +76,8 @@ def linear_w4_group(
         raise RuntimeError("x must be float16, bfloat16 or int8")
     if packed.dtype != torch.uint8 or scales.dtype != torch.float16 or packed.dim() != 2 or scales.dim() != 2:
         raise RuntimeError("packed must be uint8 [N, K/2] and scales float16 [N, K/group]")
+    if in_gemm_layout(packed) or in_gemm_layout(scales):
+        raise ValueError("this weight lies in the GEMM's order (vdm_w4a4_packed_v1): regroup_packed_weight makes a grouped one of it")
     n, k = packed.shape[0], packed.shape[1] * 2
     groups = scales.shape[1]
     if x.dim() < 1 or x.shape[-1] != k:

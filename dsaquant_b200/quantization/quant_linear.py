@@ -90,6 +90,13 @@ class QuantLinear(nn.Module):
             del self.wquantizer
             self.wquantizer = None
 
+    def _apply(self, fn, *args, **kwargs):  # .to(), .cuda(): the moved buffers are new tensors
+        super()._apply(fn, *args, **kwargs)
+        for name in ("vdm_weight_packed", "vdm_weight_scale_packed"):
+            if self._buffers.get(name) is not None:
+                _kernels().mark_gemm_layout(self._buffers[name])
+        return self
+
     # ------------------------------------------------------------------ forward
     def _forward_fake_quant(self, x: torch.Tensor) -> torch.Tensor:
         weight = self.wquantizer(self.weight) if (self.use_wq and self.wquantizer is not None) else self.weight

@@ -197,3 +197,34 @@ def test_shared_memory_of_q_and_k_is_found():
     assert _disjoint(each[:, :, 0], each[:, :, 1]) and _disjoint(each[:, :, 2], each[:, :, 0])
     assert not _disjoint(each[:, :, 0], each[:, :, 0]) and not _disjoint(by_token[:, :3], by_token[:, 2:4])
     assert _disjoint(torch.zeros(t, hq, hd), torch.zeros(t, hk, hd))
+
+
+def test_weights_in_the_gemms_order_are_known_as_such(tmp_path):
+    """The buffers of a layer read from a packed checkpoint carry their layout through moves, copies and fused projections;
+    a saved state does not."""
+    import copy
+
+    from dsaquant_b200.attention_qkv import _cat_cached
+    from dsaquant_b200.checkpoints import packed_checkpoint as pc
+    from dsaquant_b200.kernels.vdm_w4a4 import in_gemm_layout
+    from dsaquant_b200.quantization.quant_linear import QuantLinear
+
+    def loaded():
+        layer = QuantLinear(torch.nn.Linear(128, 128), {"w": "lsq", "act": "dynamic"}, {"w": {}, "act": {}})
+        pc._switch_layer_to_packed(layer, {"vdm_weight_packed": torch.zeros(128, 64, dtype=torch.uint8),
+                                           "vdm_weight_scale_packed": torch.ones(128, 2).half(), "vdm_weight_scale": torch.ones(128).half()})
+        layer._bias_half = None
+        return layer
+
+    def known(layer):
+        return in_gemm_layout(layer.vdm_weight_packed) and in_gemm_layout(layer.vdm_weight_scale_packed)
+
+    layer = loaded()
+    assert known(layer) and known(copy.deepcopy(layer)) and known(layer._apply(lambda t: t.clone()))
+    assert not in_gemm_layout(layer.vdm_weight_scale) and in_gemm_layout(layer.vdm_weight_packed[:64])
+    torch.save(layer.state_dict(), tmp_path / "layer.pt")
+    state = torch.load(tmp_path / "layer.pt", weights_only=True)
+    assert set(state) == {"bias", *pc.VDM_BUFFER_SUFFIXES} and not any(in_gemm_layout(t) for t in state.values())
+    attn, layers = torch.nn.Module(), [loaded() for _ in range(3)]
+    _cat_cached(attn, "_vdm_qkv", layers)
+    assert in_gemm_layout(attn._vdm_qkv_weight_packed) and all(known(x) for x in layers)

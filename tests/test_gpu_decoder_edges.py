@@ -4,7 +4,7 @@ test_gpu_decoder_ops."""
 import pytest
 import torch
 
-from test_gpu_decoder_ops import BF, F32, FP, HALF_STEP, HALF_SUB, _attention64, _gen, _qkv, _randn, _within
+from test_gpu_decoder_ops import BF, F32, FP, HALF_STEP, HALF_SUB, _attention64, _codes_of, _gen, _qkv, _randn, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -124,3 +124,49 @@ def test_apply_rotary_inplace_refuses_shared_memory():
     want = [apply_rotary(part.clone(), None, table, pos)[0] for part in (x[:, 2:], x[:, :2])]
     got = apply_rotary(x[:, 2:], x[:, :2], table, pos, inplace=True)          # k in front of q
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(torch.cat([want[1], want[0]], 1), x)
+
+
+# ------------------------------------------------------------------------------------------------ linear_w4_group
+def test_linear_w4_group_refuses_the_gemms_weights_and_takes_them_regrouped():
+    """A vdm_w4a4_packed_v1 weight has the shapes of a grouped one; regrouped it is the same weight, code by code."""
+    from dsaquant_b200.kernels import vdm_w4a4 as vdm
+    from dsaquant_b200.kernels.rms_norm import rms_norm_quant
+    from dsaquant_b200.kernels.w4_group import linear_w4_group, regroup_packed_weight
+    from dsaquant_b200.quantization.quant_linear import QuantLinear
+
+    g = _gen(81)
+    m, n, k = 9, 256, 1536
+    lin = torch.nn.Linear(k, n).half().cuda()
+    layer = QuantLinear(lin, {"w": "lsq", "act": "dynamic"}, {"w": {}, "act": {}})
+    layer.wquantizer.scale, layer.wquantizer.sym = (lin.weight.abs().amax(1) / 7).float(), True
+    layer.prepare_vdm_kernel_weights()
+    packed, wscales, channel = vdm.quantize_weight_per_channel(lin.weight)
+    x = _randn(g, m, k, dtype=BF)
+    codes, scale = rms_norm_quant(x, torch.ones(k, device="cuda"))
+    plain = torch.ones(n, k // 64, device="cuda", dtype=FP)
+    buffers = (layer.vdm_weight_packed, layer.vdm_weight_scale_packed)
+    w_b200, _ = vdm.prepare_b200_weight(*buffers)
+    for w, s in ((packed, wscales), (packed, plain), (torch.zeros_like(packed), wscales), buffers, (w_b200, plain)):
+        with pytest.raises(ValueError):
+            linear_w4_group(x, w, s)
+    moved = layer.cpu().cuda()
+    with pytest.raises(ValueError):
+        linear_w4_group(x, moved.vdm_weight_packed, moved.vdm_weight_scale_packed)
+
+    for qweight, ws, ch in ((packed, wscales, channel), (moved.vdm_weight_packed, moved.vdm_weight_scale_packed, moved.vdm_weight_scale)):
+        grouped = regroup_packed_weight(qweight, ch)
+        assert grouped[0].shape == (n, k // 2) and grouped[0].is_contiguous() and grouped[1].shape == (n, 1)
+        want = vdm.unpack_codes(qweight, n, k, 2)
+        assert torch.equal(_codes_of(grouped[0]), want.double())
+        y = codes.double() @ want.double().t() * scale.double()[:, None] * ch.double()
+        token = linear_w4_group(codes, *grouped, act_scale=scale)
+        prompt = vdm.linear_prequantized(codes, scale, qweight, ws)
+        # exact integer sums below 2^24 times two scales: two fp32 products (and for the matvec its sum over runs of 128,
+        # 12 terms), one rounding to fp16
+        size = codes.double().abs() @ want.double().abs().t() * scale.double()[:, None] * ch.double()
+        for got in (token, prompt):
+            _within(got, y, 2.0 ** -11 * y.abs() + 2.0 ** -25 + 28 * 2.0 ** -24 * size)
+    for bad in (lambda: regroup_packed_weight(packed[:100], channel[:100]), lambda: regroup_packed_weight(packed, channel.float()),
+                lambda: regroup_packed_weight(packed, channel[:128]), lambda: regroup_packed_weight(packed.to(torch.int8), channel)):
+        with pytest.raises(ValueError):
+            bad()
