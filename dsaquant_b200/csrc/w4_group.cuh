@@ -32,6 +32,8 @@
 
 #include <type_traits>
 
+#include "rms_norm.cuh"  // max_nan
+
 namespace b200w4a4 {
 
 struct W4GroupArgs {
@@ -301,16 +303,20 @@ inline cudaError_t launch_w4_group(const W4GroupArgs& a, int sm_count, cudaStrea
   return launch_w4_group_tile<X, GB, 2, 4, 2>(a, sm_count, stream);
 }
 
-// ---- quantiser (load time): scale = max(absmax, 1e-5) / 7 in fp16, code = clamp(rint(w / scale), -8, 7)
+// ---- quantiser (load time): scale = max(absmax, 1e-5) / 7 in fp16, code = clamp(rint(w / scale), -8, 7).  A group that holds a
+// NaN or an infinity, or whose scale passes fp16's range, has scale NaN and codes 0, so that every product with it shows.
 template <typename W>
 __global__ void w4_group_scale_kernel(const W* __restrict__ w, __half* __restrict__ scale, long long groups, int group) {
   const long long i = static_cast<long long>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32;
   if (i >= groups) return;
   float m = 0.0f;
-  for (int k = threadIdx.x & 31; k < group; k += 32) m = fmaxf(m, fabsf(static_cast<float>(w[i * group + k])));
+  for (int k = threadIdx.x & 31; k < group; k += 32) m = detail::max_nan(m, fabsf(static_cast<float>(w[i * group + k])));
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if ((threadIdx.x & 31) == 0) scale[i] = __float2half_rn(fminf(__fdiv_rn(fmaxf(m, 1e-5f), 7.0f), 65504.0f));
+  for (int o = 16; o > 0; o >>= 1) m = detail::max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((threadIdx.x & 31) == 0) {
+    const __half s = __float2half_rn(__fdiv_rn(detail::max_nan(m, 1e-5f), 7.0f));
+    scale[i] = __half2float(s) < INFINITY ? s : __ushort_as_half(0x7fff);
+  }
 }
 template <typename W>
 __global__ void w4_group_pack_kernel(const W* __restrict__ w, const __half* __restrict__ scale, uint8_t* __restrict__ packed,
@@ -321,7 +327,7 @@ __global__ void w4_group_pack_kernel(const W* __restrict__ w, const __half* __re
   uint32_t b = 0;
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    const float t = fminf(fmaxf(__fdiv_rn(static_cast<float>(w[2 * i + e]), s), -8.0f), 7.0f);
+    const float t = isnan(s) ? 0.0f : fminf(fmaxf(__fdiv_rn(static_cast<float>(w[2 * i + e]), s), -8.0f), 7.0f);
     b |= (static_cast<uint32_t>(__float2int_rn(t)) & 15u) << (4 * e);
   }
   packed[i] = static_cast<uint8_t>(b);

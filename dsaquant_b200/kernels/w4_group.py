@@ -25,7 +25,8 @@ _OUT_CODE = {torch.float16: 0, torch.bfloat16: 1}
 
 def quantize_weight_grouped(weight: torch.Tensor, group_size: int = 128) -> Tuple[torch.Tensor, torch.Tensor]:
     """fp weight [N, K] -> (packed, scales): scale = max(absmax, 1e-5) / 7 of each group in fp16,
-    code = clamp(rint(w / scale), -8, 7)."""
+    code = clamp(rint(w / scale), -8, 7).  A group that holds a NaN or an infinity, or a value past 458000 (its scale would
+    pass fp16's range), has scale NaN and codes 0: outputs of that row are NaN."""
     lib = _load_ext()
     _require_cuda(weight, "weight")
     if weight.dtype not in _DTYPE_CODE or weight.dim() != 2:

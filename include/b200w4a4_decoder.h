@@ -36,7 +36,8 @@ int b200w4a4_rms_norm_quant(const void* x, int x_dtype, long long x_ld, const vo
 
 /* w [N, K] (F16, BF16, F32, contiguous) -> packed u8 [N, K/2] (code 2b in the low nibble, 2b+1 in the
  * high one, two's complement) and scale f16 [N, K/group] = max(absmax, 1e-5) / 7 of each run of
- * `group` values; code = clamp(rint(w / scale), -8, 7).  group: a multiple of 32 that divides K. */
+ * `group` values; code = clamp(rint(w / scale), -8, 7).  group: a multiple of 32 that divides K.
+ * A group that is not finite, or whose scale passes fp16's range, gets scale NaN and codes 0. */
 int b200w4a4_quantize_weight_grouped(const void* w, int w_dtype, void* packed, void* scale, int N,
                                      int K, int group, void* stream);
 

@@ -170,3 +170,41 @@ def test_linear_w4_group_refuses_the_gemms_weights_and_takes_them_regrouped():
                 lambda: regroup_packed_weight(packed, channel[:128]), lambda: regroup_packed_weight(packed.to(torch.int8), channel)):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf"), 1e6])
+def test_quantize_weight_grouped_marks_groups_that_are_not_finite(dtype, value):
+    """A weight that is not finite, or too large for an fp16 scale, shows in the scale and in every product, and leaves the other
+    groups as they are."""
+    from dsaquant_b200.kernels.w4_group import linear_w4_group, quantize_weight_grouped
+
+    g = _gen(91)
+    n, k, group = 40, 512, 64
+    w = (_randn(g, n, k) * 0.02).to(dtype)
+    packed, scales = quantize_weight_grouped(w, group)
+    for row, col in ((0, 0), (17, 130), (39, 511)):
+        w[row, col] = value                                          # 1e6 is an infinity in fp16
+    got, got_scales = quantize_weight_grouped(w, group)
+    hit = torch.zeros(n, k // group, dtype=torch.bool, device="cuda")
+    hit[0, 0] = hit[17, 2] = hit[39, 7] = True
+    assert bool(torch.isnan(got_scales[hit]).all()) and torch.equal(got_scales[~hit], scales[~hit])
+    parts, want = got.view(n, k // group, -1), packed.view(n, k // group, -1)
+    assert bool((parts[hit] == 0).all()) and torch.equal(parts[~hit], want[~hit])
+    x = _randn(g, 3, k, dtype=BF)
+    y, clean = linear_w4_group(x, got, got_scales), linear_w4_group(x, packed, scales)
+    rows = hit.any(1)
+    assert bool(torch.isnan(y[:, rows]).all()) and torch.equal(y[:, ~rows], clean[:, ~rows])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_quantize_weight_grouped_largest_scale(dtype):
+    """The largest weight whose scale fp16 holds keeps its value; the next power of two marks the group."""
+    from dsaquant_b200.kernels.w4_group import quantize_weight_grouped
+
+    w = torch.zeros(2, 32, device="cuda", dtype=dtype)
+    w[0, 3], w[1, 3] = 65504.0 * 7, 65536.0 * 7                      # 458752 = 7 * 2^16; bf16 rounds the first up to it
+    packed, scales = quantize_weight_grouped(w, 32)
+    assert bool(torch.isnan(scales[1]).all())
+    if dtype == F32:
+        assert scales[0].item() == 65504.0 and _codes_of(packed)[0, 3].item() == 7
