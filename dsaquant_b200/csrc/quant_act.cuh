@@ -135,11 +135,12 @@ __device__ __forceinline__ float row_scale(float amax, float clip) {
   return __fmul_rn(__fdiv_rn(fmaxf(amax, 1e-5f), 7.0f), clip);
 }
 
-// Bits of (clamp(rint(x / s), -8, 7) + magic): the code is the low byte (two's complement).
-// Clamping first is equivalent because the bounds are integers.
+// Bits of (clamp(rint(x / s), -TOP - 1, TOP) + magic), TOP = 7 or 127: the code is the low byte (two's
+// complement).  Clamping first is equivalent because the bounds are integers.
+template <int TOP = 7>
 __device__ __forceinline__ uint32_t code_bits_div(float x, float s) {
   float t = __fdiv_rn(x, s);
-  t = fminf(fmaxf(t, -8.0f), 7.0f);
+  t = fminf(fmaxf(t, -TOP - 1.0f), static_cast<float>(TOP));
   return __float_as_uint(t + kRoundMagic);
 }
 
@@ -148,7 +149,7 @@ struct RowQuant {
   float s;          // scale
   float r_up, r_dn; // RN(1/s) nudged up / down by 2^-20: brackets of the true reciprocal
   bool exact_only;  // scale so large or small that 1/s is not a normal number: always divide
-  bool clamp;       // |x/s| can exceed 7.5 (clip below ~0.934): clamp the rounded values
+  bool clamp;       // |x/s| can exceed TOP + 1/2 (for 7: clip below ~0.934): clamp the rounded values
 };
 
 // Eight codes of one chunk.  Fast path: two fused multiply-adds per value,
@@ -159,7 +160,7 @@ struct RowQuant {
 // each; rint is monotonic, so ya == yb implies rint(fl(x/s)) == ya.  When they differ somewhere
 // in the chunk (a value within ~2^-16 of a rounding tie: a few chunks per hundred thousand) the
 // chunk is redone with the IEEE division, so the result equals clamp(rint(x / s)) for every input.
-template <bool CLAMP>
+template <bool CLAMP, int TOP = 7>
 __device__ __forceinline__ uint32_t chunk_codes_fast(const float (&v)[8], const RowQuant& rq, uint32_t (&c)[8]) {
   uint32_t diff = 0;
 #pragma unroll
@@ -167,8 +168,8 @@ __device__ __forceinline__ uint32_t chunk_codes_fast(const float (&v)[8], const 
     float ya = __fmaf_rn(v[i], rq.r_up, kRoundMagic);
     float yb = __fmaf_rn(v[i], rq.r_dn, kRoundMagic);
     if constexpr (CLAMP) {
-      ya = fminf(fmaxf(ya, kRoundMagic - 8.0f), kRoundMagic + 7.0f);
-      yb = fminf(fmaxf(yb, kRoundMagic - 8.0f), kRoundMagic + 7.0f);
+      ya = fminf(fmaxf(ya, kRoundMagic - TOP - 1.0f), kRoundMagic + TOP);
+      yb = fminf(fmaxf(yb, kRoundMagic - TOP - 1.0f), kRoundMagic + TOP);
     }
     diff |= __float_as_uint(ya) ^ __float_as_uint(yb);
     c[i] = __float_as_uint(ya);
@@ -176,12 +177,13 @@ __device__ __forceinline__ uint32_t chunk_codes_fast(const float (&v)[8], const 
   return diff;
 }
 
+template <int TOP = 7>
 __device__ __forceinline__ void chunk_codes(const float (&v)[8], const RowQuant& rq, uint32_t (&c)[8]) {
   // rq.clamp is the same for the whole launch: two straight-line bodies, one uniform branch.
-  const uint32_t diff = rq.clamp ? chunk_codes_fast<true>(v, rq, c) : chunk_codes_fast<false>(v, rq, c);
+  const uint32_t diff = rq.clamp ? chunk_codes_fast<true, TOP>(v, rq, c) : chunk_codes_fast<false, TOP>(v, rq, c);
   if (rq.exact_only || diff != 0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = code_bits_div(v[i], rq.s);
+    for (int i = 0; i < 8; ++i) c[i] = code_bits_div<TOP>(v[i], rq.s);
   }
 }
 
@@ -202,17 +204,20 @@ __device__ __forceinline__ void store_codes(void* q, size_t row, int K, int chun
   }
 }
 
-__device__ __forceinline__ RowQuant row_quant(float amax, float clip) {
+// s: the row's scale; clip: what its step was multiplied by (|x| <= amax gives |x/s| <= TOP / clip, and rounding
+// stays within [-TOP, TOP] while that is below TOP + 1/2).
+template <int TOP = 7>
+__device__ __forceinline__ RowQuant row_quant_of(float s, float clip) {
   RowQuant rq;
-  rq.s = row_scale(amax, clip);
+  rq.s = s;
   rq.exact_only = !(rq.s < 1.0e30f) || !(rq.s > 1.0e-30f);  // also true for NaN / inf scales
   const float r = rq.exact_only ? 0.0f : __frcp_rn(rq.s);
   rq.r_up = __fmul_rn(r, 1.0f + 9.5367431640625e-07f);  // 1 + 2^-20
   rq.r_dn = __fmul_rn(r, 1.0f - 9.5367431640625e-07f);
-  // |x| <= amax gives |x/s| <= 7/clip; rounding stays within [-7, 7] while that is below 7.5.
-  rq.clamp = !(clip >= 0.934f);
+  rq.clamp = !(clip >= (TOP == 7 ? 0.934f : 0.997f));
   return rq;
 }
+__device__ __forceinline__ RowQuant row_quant(float amax, float clip) { return row_quant_of(row_scale(amax, clip), clip); }
 
 }  // namespace detail
 

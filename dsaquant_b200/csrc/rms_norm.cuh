@@ -90,9 +90,6 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-__device__ __forceinline__ uint32_t code_int8(float y, float inv) {
-  return __float_as_uint(fminf(fmaxf(y * inv, -128.0f), 127.0f) + kRoundMagic);  // low byte
-}
 // distance of a positive quotient's bits from the first pattern 16 steps below an e4m3 midpoint: under 32 near one
 __device__ __forceinline__ uint32_t past_midpoint(float t) { return (__float_as_uint(t) - 0x7fff0u) & 0xfffffu; }
 // the e4m3 value nearest to num / den (den > 0), a quotient near a midpoint; compared without dividing, so ties are seen
@@ -215,7 +212,8 @@ __global__ void __launch_bounds__(256, NCH <= 5 ? 4 : 2) rms_norm_quant_kernel(c
   const bool good = ss < INFINITY && amax < INFINITY;  // false for NaN
   const float top = E4M3 ? 448.0f : 127.0f;
   const float s = __fmul_rn(__fdiv_rn(fmaxf(amax, 1e-5f), top), a.clip);
-  const float inv = __fdiv_rn(1.0f, s);
+  [[maybe_unused]] const float inv = E4M3 ? __fdiv_rn(1.0f, s) : 0.0f;
+  [[maybe_unused]] const detail::RowQuant rq = detail::row_quant_of<127>(s, a.clip);
   uint8_t* q = static_cast<uint8_t*>(a.codes) + (row_ok ? row : 0) * a.D;
   // e4m3: which of this thread's values are the row's largest, and which lie near a midpoint
   constexpr int MW = E4M3 ? (NCH + 3) / 4 : 1;
@@ -233,6 +231,8 @@ __global__ void __launch_bounds__(256, NCH <= 5 ? 4 : 2) rms_norm_quant_kernel(c
   if (row_ok && t == 0) a.scale[row] = good ? s : __int_as_float(0x7fc00000);
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
+    [[maybe_unused]] uint32_t c[8];  // int8 codes: low bytes
+    if constexpr (!E4M3) detail::chunk_codes<127>(v[i], rq, c);
     if constexpr (VEC) {
       if (at(i, 0) >= a.D) continue;
       uint2 o = make_uint2(0u, 0u);
@@ -241,9 +241,6 @@ __global__ void __launch_bounds__(256, NCH <= 5 ? 4 : 2) rms_norm_quant_kernel(c
           o.x = detail::code_e4m3x2(v[i][0], v[i][1]) | detail::code_e4m3x2(v[i][2], v[i][3]) << 16;
           o.y = detail::code_e4m3x2(v[i][4], v[i][5]) | detail::code_e4m3x2(v[i][6], v[i][7]) << 16;
         } else {
-          uint32_t c[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) c[e] = detail::code_int8(v[i][e], inv);
           o.x = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
           o.y = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
         }
@@ -253,9 +250,10 @@ __global__ void __launch_bounds__(256, NCH <= 5 ? 4 : 2) rms_norm_quant_kernel(c
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         if (at(i, e) >= a.D) continue;
-        uint32_t c = 0;
-        if (good) c = E4M3 ? detail::code_e4m3x2(v[i][e], 0.0f) : detail::code_int8(v[i][e], inv);
-        if (row_ok) q[at(i, e)] = static_cast<uint8_t>(c);
+        uint32_t code = 0;
+        if constexpr (E4M3) code = detail::code_e4m3x2(v[i][e], 0.0f);
+        else code = c[e];
+        if (row_ok) q[at(i, e)] = static_cast<uint8_t>(good ? code : 0u);
       }
     }
   }

@@ -39,6 +39,27 @@ def test_rms_norm_quant_e4m3_short_rows_share_a_block(d, dtype):
     assert torch.equal(codes.double()[normal], _nearest_e4m3(t)[normal])
 
 
+@pytest.mark.parametrize("d, clip", [(512, 1.0), (5120, 1.0), (777, 0.9), (64, 0.5)])
+def test_rms_norm_quant_int8_codes_are_those_of_the_division(d, clip):
+    """codes = clamp(rint(y / scale)) with fp32's quotient, as the package's other quantiser rounds, at quotients beside the
+    borders.  Squares far below eps = 1 leave rsqrt(1) = 1, so y is x."""
+    from dsaquant_b200.kernels.rms_norm import rms_norm_quant
+
+    g = _gen(55 + d)
+    m = 1_000_000 // d
+    top = (1 + torch.rand(m, 1, generator=g, device="cuda")) * 2.0 ** -15
+    scale = (top / torch.full_like(top, 127.0)) * torch.tensor(clip, device="cuda")   # (by a number torch multiplies with 1 / 127)
+    half = torch.randint(-128, 128, (m, d), generator=g, device="cuda") + 0.5
+    x = half * scale
+    x = (x.view(torch.int32) + torch.randint(-1, 2, (m, d), generator=g, device="cuda", dtype=torch.int32)).view(F32)
+    x = torch.minimum(torch.maximum(x, -top), top)
+    x[:, d // 2] = top[:, 0]
+    assert x.square().mean(-1).max().item() < 2.0 ** -25
+    codes, got_scale = rms_norm_quant(x, torch.ones(d, device="cuda"), 1.0, clip_ratio=clip)
+    assert torch.equal(got_scale, scale[:, 0])
+    assert torch.equal(codes.float(), (x / scale).round().clamp(-128, 127))
+
+
 # ------------------------------------------------------------------------------------------------ window_attention
 def _attention_bound(q, k, v, window, sinks, lens):
     """The definition in 64 bits and how far a result may be off (the terms are explained at _check_attention)."""
