@@ -109,14 +109,16 @@ int b200w4a4_linear_w4_group(const void* x, int x_dtype, const float* act_scale,
                              const void* scale, const void* bias, void* out, int out_dtype, int M,
                              int N, int K, int group, void* stream) {
   if (x_dtype != B200W4A4_F16 && x_dtype != B200W4A4_BF16 && x_dtype != B200W4A4_X_INT8) return B200W4A4_EINVAL;
+  const bool bias_f32 = (out_dtype & B200W4A4_BIAS_F32) != 0;
+  out_dtype &= ~B200W4A4_BIAS_F32;
   if (out_dtype != B200W4A4_F16 && out_dtype != B200W4A4_BF16) return B200W4A4_EINVAL;
   if (M < 0 || N < 1 || K < 32 || group < 32 || group % 32 != 0 || K % group != 0) return B200W4A4_ESHAPE;
   if (M > 65535 * 8 || K > (1 << 20)) return B200W4A4_ESHAPE;
   if (M == 0) return B200W4A4_OK;
   if (x == nullptr || packed == nullptr || scale == nullptr || out == nullptr) return B200W4A4_EINVAL;
   if ((x_dtype == B200W4A4_X_INT8) != (act_scale != nullptr)) return B200W4A4_EINVAL;
-  if (!aligned(x, 16) || !aligned(packed, 16) || !aligned(scale, 2) || !aligned(out, 2) || !aligned(bias, 2) ||
-      !aligned(act_scale, 4))
+  if (!aligned(x, 16) || !aligned(packed, 16) || !aligned(scale, 2) || !aligned(out, 2) ||
+      !aligned(bias, bias_f32 ? 4 : 2) || !aligned(act_scale, 4))
     return B200W4A4_EALIGN;
   DeviceInfo dev;
   const int rc = current_device(&dev);
@@ -126,7 +128,8 @@ int b200w4a4_linear_w4_group(const void* x, int x_dtype, const float* act_scale,
   a.packed = static_cast<const uint8_t*>(packed);
   a.scale = static_cast<const __half*>(scale);
   a.act_scale = act_scale;
-  a.bias = bias;
+  a.bias = bias_f32 ? nullptr : bias;
+  a.bias32 = bias_f32 ? static_cast<const float*>(bias) : nullptr;
   a.out = out;
   a.M = M;
   a.N = N;

@@ -41,7 +41,8 @@ struct W4GroupArgs {
   const uint8_t* packed;   // [N, K/2]
   const __half* scale;     // [N, K/group]
   const float* act_scale;  // [M] (int8 x) or null
-  const void* bias;        // [N] of the output type or null
+  const void* bias;        // [N] of the output type, or null
+  const float* bias32;     // [N] fp32, or null
   void* out;               // [M, N]
   int M, N, K, group;
   int group_runs;          // group / GB (set by the launcher), and the multiplier that divides by it:
@@ -268,6 +269,7 @@ __global__ void __launch_bounds__(32 * kW4Warps, NT == 4 ? 1 : 3) w4_group_kerne
     for (int v = 0; v < split; ++v) y += total[tile * split + v][in_tile][n];
     if (a.act_scale != nullptr) y *= a.act_scale[tok];
     const long long o = static_cast<long long>(tok) * a.N + row;
+    if (a.bias32 != nullptr) y += a.bias32[row];
     if (a.out_bf16) {
       if (a.bias != nullptr) y += __bfloat162float(static_cast<const __nv_bfloat16*>(a.bias)[row]);
       static_cast<__nv_bfloat16*>(a.out)[o] = __float2bfloat16_rn(y);

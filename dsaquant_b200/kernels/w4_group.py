@@ -21,6 +21,7 @@ from .vdm_w4a4 import _DTYPE_CODE, _empty, _load_ext, _require_cuda, _run, _stre
 _X_CODE = {torch.float16: 0, torch.bfloat16: 1, torch.int8: 3}
 MAX_TOKENS = 65535 * 8
 _OUT_CODE = {torch.float16: 0, torch.bfloat16: 1}
+_BIAS_F32 = 16
 
 
 def quantize_weight_grouped(weight: torch.Tensor, group_size: int = 128) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -68,7 +69,8 @@ def linear_w4_group(
 ) -> torch.Tensor:
     """x [..., K] times the grouped 4-bit weight, plus bias [N]: [..., N].  x is fp16 or bf16 (multiplied as it is,
     fp32 sums), or int8 codes with act_scale, their fp32 scale per token, as `rms_norm_quant` and
-    `quantize_activation_per_token` return them.  out_dtype: fp16 or bf16, by default x's (fp16 for int8).
+    `quantize_activation_per_token` return them.  out_dtype: fp16 or bf16, by default x's (fp16 for int8).  The bias is
+    added in fp32, whatever its type, before the one rounding to out_dtype.
     For single tokens and small batches: the weight is read once for every 8 to 32 tokens, and any number of
     tokens is right, but from some hundreds on a GEMM is faster."""
     lib = _load_ext()
@@ -106,17 +108,20 @@ def linear_w4_group(
         if act_scale.dtype != torch.float32 or act_scale.numel() != m or act_scale.device != dev:
             raise ValueError("act_scale must be float32 with one value for each token")
         act_scale = act_scale.contiguous()
+    out_code = _OUT_CODE[out_dtype]
     if bias is not None:
         if bias.numel() != n or bias.device != dev:
             raise ValueError("bias must have N elements")
-        if bias.dtype != out_dtype or not bias.is_contiguous():
-            bias = bias.detach().to(out_dtype).contiguous()
+        if bias.dtype != out_dtype:  # added before the one rounding to the output's type, as it is
+            bias = bias.float()
+            out_code |= _BIAS_F32
+        bias = bias.contiguous()
     out = _empty((*x.shape[:-1], n), out_dtype, dev)
     if m > 0:
         rc = _run(
             dev, lib.b200w4a4_linear_w4_group, x2.data_ptr(), _X_CODE[x.dtype],
             act_scale.data_ptr() if act_scale is not None else None, packed.data_ptr(), scales.data_ptr(),
-            bias.data_ptr() if bias is not None else None, out.data_ptr(), _OUT_CODE[out_dtype], m, n, k, k // groups,
+            bias.data_ptr() if bias is not None else None, out.data_ptr(), out_code, m, n, k, k // groups,
             _stream_ptr(dev))
         _lib.check(rc, "linear_w4_group")
     return out

@@ -228,3 +228,8 @@ def test_weights_in_the_gemms_order_are_known_as_such(tmp_path):
     attn, layers = torch.nn.Module(), [loaded() for _ in range(3)]
     _cat_cached(attn, "_vdm_qkv", layers)
     assert in_gemm_layout(attn._vdm_qkv_weight_packed) and all(known(x) for x in layers)
+
+
+@pytest.mark.parametrize("over, code", [(dict(odt=16, bias=P + 2), -3), (dict(odt=18), -1), (dict(odt=17, m=0), 0), (dict(odt=32), -1)])
+def test_linear_w4_group_fp32_bias_refusals(lib, over, code):
+    assert _w4(lib, **over) == code

@@ -4,7 +4,7 @@ test_gpu_decoder_ops."""
 import pytest
 import torch
 
-from test_gpu_decoder_ops import BF, F32, FP, HALF_STEP, HALF_SUB, _attention64, _codes_of, _gen, _qkv, _randn, _within
+from test_gpu_decoder_ops import BF, F32, FP, HALF_STEP, HALF_SUB, _attention64, _check_w4, _codes_of, _gen, _qkv, _randn, _w4_case, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -229,3 +229,18 @@ def test_quantize_weight_grouped_largest_scale(dtype):
     assert bool(torch.isnan(scales[1]).all())
     if dtype == F32:
         assert scales[0].item() == 65504.0 and _codes_of(packed)[0, 3].item() == 7
+
+
+@pytest.mark.parametrize("xdtype, out_dtype", [(BF, BF), (FP, FP), (torch.int8, FP), (torch.int8, BF)])
+@pytest.mark.parametrize("bias_dtype", [BF, FP, F32, torch.float64])
+def test_linear_w4_group_adds_the_bias_as_it_is(xdtype, out_dtype, bias_dtype):
+    """A bias of another type than the output is not rounded to it before the addition."""
+    g = _gen(95)
+    packed, scales = _w4_case(g, 300, 256, 64)
+    bias = (100 + _randn(g, 300)).to(bias_dtype)                     # its rounding to 16 bits would outweigh the sums
+    act = None
+    x = _randn(g, 5, 256, dtype=BF if xdtype == torch.int8 else xdtype) * 0.1
+    if xdtype == torch.int8:
+        x, act = (x * 100).round().clamp(-128, 127).to(torch.int8), torch.full((5,), 0.001, device="cuda")
+    _check_w4(x, packed, scales, bias, act, out_dtype)
+    _check_w4(x, packed, scales, bias.repeat_interleave(2)[::2], act, out_dtype)
