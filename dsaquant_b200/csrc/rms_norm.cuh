@@ -13,7 +13,8 @@
 // e4m3 codes are those of the exact quotient: its midpoints are 2^-4 of a value apart, so among millions of values
 // some always lie within the fp32 roundings of one, and a code on the wrong side is a step of 6 %.  A value whose
 // quotient lies within 16 fp32 steps of a midpoint (one in 2^15) is read again and decided in 64 bits, against the
-// row's largest |s * weight|, of which 64 bits are kept too; the rsqrt cancels.
+// row's largest |s * weight|, of which 64 bits are kept too; the rsqrt cancels.  The largest is sought among all values
+// within 2^-20 of the fp32 maximum, whose order three roundings each may have changed (2^-21.4).
 //
 // A row whose sum of squares or whose y is not finite has no meaningful codes: its scale is NaN
 // (whatever is computed from it shows it) and its codes are 0.
@@ -219,11 +220,12 @@ __global__ void __launch_bounds__(256, NCH <= 5 ? 4 : 2) rms_norm_quant_kernel(c
   constexpr int MW = E4M3 ? (NCH + 3) / 4 : 1;
   uint32_t largest[MW] = {}, near[MW] = {};
   if constexpr (E4M3) {
+    const float near_top = amax * 0.99999905f;  // 1 - 2^-20
 #pragma unroll
     for (int i = 0; i < NCH; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        if (fabsf(v[i][e]) == amax) largest[i / 4] |= 1u << (8 * (i % 4) + e);
+        if (fabsf(v[i][e]) >= near_top) largest[i / 4] |= 1u << (8 * (i % 4) + e);
         v[i][e] = fminf(fmaxf(v[i][e] * inv, -448.0f), 448.0f);
         if (detail::past_midpoint(v[i][e]) < 32) near[i / 4] |= 1u << (8 * (i % 4) + e);
       }

@@ -39,6 +39,38 @@ def test_rms_norm_quant_e4m3_short_rows_share_a_block(d, dtype):
     assert torch.equal(codes.double()[normal], _nearest_e4m3(t)[normal])
 
 
+def test_rms_norm_quant_e4m3_largest_value_in_64_bits():
+    """Two values so close that their fp32 products come out in the wrong order, and quotients that lie on one side of a
+    border for one of them and on the other side for the other.  Rows of whole numbers, whose squares add up exactly."""
+    from dsaquant_b200.kernels.rms_norm import rms_norm_quant
+
+    g = _gen(53)
+    rows, d, found = 200_000, 32, 0
+    x = torch.randint(129, 256, (rows, d), generator=g, device="cuda").float()
+    w = 1 + torch.rand(rows, d, generator=g, device="cuda")
+    w[:, 0] += 64                                                    # values 0 and 1 are the largest by far
+    # torch's root may differ from the kernel's in the last bit; then a row is only not as hard as it was meant to be
+    rstd = torch.rsqrt(x.square().mean(-1) + 1e-6)
+    w[:, 1] = (x[:, 0].double() * w[:, 0].double() / x[:, 1].double()).float()
+    w[:, 1] = (w[:, 1].view(torch.int32) + 1).view(F32)              # the true maximum is value 1
+    top = x[:, 1].double() * w[:, 1].double()
+    fp32 = x * rstd[:, None] * w
+    wrong = (top > x[:, 0].double() * w[:, 0].double()) & (fp32[:, 1] < fp32[:, 0])
+    for j in range(2, d):                                            # quotients as near to a border as fp32 weights allow
+        border = 1.0625 * 2.0 ** (j % 6) + 0.125 * 2.0 ** (j % 6) * (j % 7)
+        w[:, j] = (border * top / (448 * x[:, j].double())).float()
+    for row in wrong.nonzero()[:, 0][:300].tolist():
+        y = x[row].double() * w[row].double()
+        t, t0 = y * 448 / y.abs().amax(), y * 448 / y[0].abs()
+        want, with_other = _nearest_e4m3(t.clamp(max=448.0)), _nearest_e4m3(t0.clamp(max=448.0))
+        if torch.equal(want, with_other):
+            continue
+        found += 1
+        codes, _ = rms_norm_quant(x[row:row + 1], w[row], out_dtype=torch.float8_e4m3fn)
+        assert torch.equal(codes[0].double(), want)
+    assert found > 10
+
+
 @pytest.mark.parametrize("d, clip", [(512, 1.0), (5120, 1.0), (777, 0.9), (64, 0.5)])
 def test_rms_norm_quant_int8_codes_are_those_of_the_division(d, clip):
     """codes = clamp(rint(y / scale)) with fp32's quotient, as the package's other quantiser rounds, at quotients beside the
