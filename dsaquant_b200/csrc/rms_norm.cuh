@@ -11,8 +11,10 @@
 // allows no 128-bit access move one value an access: 20000 x 5121 with residual 445 us, four times the copy.
 //
 // e4m3 codes are those of the exact quotient: its midpoints are 2^-4 of a value apart, so among millions of values
-// some always lie within the fp32 roundings of one, and a code on the wrong side is a step of 6 %.  A value whose
-// quotient lies within 16 fp32 steps of a midpoint (one in 2^15) is read again and decided in 64 bits, against the
+// some always lie within the fp32 roundings of one, and a code on the wrong side is a step of 6 %.  So every value is
+// converted twice, with the reciprocal of the scale nudged up and down by 2^-20; the roundings on the way to a quotient (s and
+// two products, the same for the largest value, scale, reciprocal, product: ten halves of 2^-23) are less.  A value with two
+// codes (one in 2^15) is read again and decided in 64 bits, against the
 // row's largest |s * weight|, of which 64 bits are kept too; the rsqrt cancels.  The largest is sought among all values
 // within 2^-20 of the fp32 maximum, whose order three roundings each may have changed (2^-21.4).
 //
@@ -91,15 +93,26 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// distance of a positive quotient's bits from the first pattern 16 steps below an e4m3 midpoint: under 32 near one
-__device__ __forceinline__ uint32_t past_midpoint(float t) { return (__float_as_uint(t) - 0x7fff0u) & 0xfffffu; }
 // the e4m3 value nearest to num / den (den > 0), a quotient near a midpoint; compared without dividing, so ties are seen
 __device__ __forceinline__ float nearest_e4m3(double num, double den) {
-  const float t = static_cast<float>(fabs(num) / den);
-  const uint32_t low = (__float_as_uint(t) - 32u) & 0xfff00000u;  // the lower neighbour
-  const double mid = static_cast<double>(__uint_as_float(low | 0x80000u)) * den, a = fabs(num);
-  const bool up = a > mid || (a == mid && (low & 0x100000u) != 0);  // ties to the even one
-  return copysignf(__uint_as_float(up ? low + 0x100000u : low), static_cast<float>(num));
+  const double a = fabs(num);
+  const float t = static_cast<float>(a / den);
+  float low, next;  // the neighbours
+  bool odd;
+  if (t < 0.015625f) {  // steps of 2^-9
+    const float step = floorf(t * 512.0f);
+    low = step * 0.001953125f;
+    next = (step + 1.0f) * 0.001953125f;
+    odd = (static_cast<int>(step) & 1) != 0;
+  } else {
+    const uint32_t bits = __float_as_uint(t) & 0xfff00000u;
+    low = __uint_as_float(bits);
+    next = __uint_as_float(bits + 0x100000u);
+    odd = (bits & 0x100000u) != 0;
+  }
+  const double mid = 0.5 * (static_cast<double>(low) + static_cast<double>(next)) * den;
+  const bool up = a > mid || (a == mid && odd);  // ties to the even one
+  return copysignf(up ? next : low, static_cast<float>(num));
 }
 __device__ __forceinline__ uint32_t code_e4m3x2(float lo, float hi) {
   return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
@@ -213,35 +226,49 @@ __global__ void __launch_bounds__(256, NCH <= 5 ? 4 : 2) rms_norm_quant_kernel(c
   const bool good = ss < INFINITY && amax < INFINITY;  // false for NaN
   const float top = E4M3 ? 448.0f : 127.0f;
   const float s = __fmul_rn(__fdiv_rn(fmaxf(amax, 1e-5f), top), a.clip);
-  [[maybe_unused]] const float inv = E4M3 ? __fdiv_rn(1.0f, s) : 0.0f;
+  [[maybe_unused]] float inv_up = 0.0f, inv_dn = 0.0f;
+  if constexpr (E4M3) {
+    const float inv = __fdiv_rn(1.0f, s);
+    inv_up = inv * 1.00000095f;  // 1 + 2^-20
+    inv_dn = inv * 0.99999905f;
+  }
   [[maybe_unused]] const detail::RowQuant rq = detail::row_quant_of<127>(s, a.clip);
   uint8_t* q = static_cast<uint8_t*>(a.codes) + (row_ok ? row : 0) * a.D;
-  // e4m3: which of this thread's values are the row's largest, and which lie near a midpoint
+  // e4m3: which of this thread's values may be the row's largest, and which lie near a midpoint
   constexpr int MW = E4M3 ? (NCH + 3) / 4 : 1;
   uint32_t largest[MW] = {}, near[MW] = {};
-  if constexpr (E4M3) {
-    const float near_top = amax * 0.99999905f;  // 1 - 2^-20
-#pragma unroll
-    for (int i = 0; i < NCH; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (fabsf(v[i][e]) >= near_top) largest[i / 4] |= 1u << (8 * (i % 4) + e);
-        v[i][e] = fminf(fmaxf(v[i][e] * inv, -448.0f), 448.0f);
-        if (detail::past_midpoint(v[i][e]) < 32) near[i / 4] |= 1u << (8 * (i % 4) + e);
-      }
-  }
+  [[maybe_unused]] const float near_top = amax * 0.99999905f;
   if (row_ok && t == 0) a.scale[row] = good ? s : __int_as_float(0x7fc00000);
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
     [[maybe_unused]] uint32_t c[8];  // int8 codes: low bytes
-    if constexpr (!E4M3) detail::chunk_codes<127>(v[i], rq, c);
+    [[maybe_unused]] uint32_t up[2];  // e4m3 codes, four a word
+    if constexpr (E4M3) {
+      uint32_t apart = 0, dn[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float* u = v[i] + 4 * h;
+        up[h] = detail::code_e4m3x2(u[0] * inv_up, u[1] * inv_up) | detail::code_e4m3x2(u[2] * inv_up, u[3] * inv_up) << 16;
+        dn[h] = detail::code_e4m3x2(u[0] * inv_dn, u[1] * inv_dn) | detail::code_e4m3x2(u[2] * inv_dn, u[3] * inv_dn) << 16;
+        apart |= up[h] ^ dn[h];
+      }
+      if (apart != 0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if ((up[e / 4] ^ dn[e / 4]) >> (8 * (e % 4)) & 0xff) near[i / 4] |= 1u << (8 * (i % 4) + e);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (fabsf(v[i][e]) >= near_top) largest[i / 4] |= 1u << (8 * (i % 4) + e);
+    } else {
+      detail::chunk_codes<127>(v[i], rq, c);
+    }
     if constexpr (VEC) {
       if (at(i, 0) >= a.D) continue;
       uint2 o = make_uint2(0u, 0u);
       if (good) {
         if constexpr (E4M3) {
-          o.x = detail::code_e4m3x2(v[i][0], v[i][1]) | detail::code_e4m3x2(v[i][2], v[i][3]) << 16;
-          o.y = detail::code_e4m3x2(v[i][4], v[i][5]) | detail::code_e4m3x2(v[i][6], v[i][7]) << 16;
+          o = make_uint2(up[0], up[1]);
         } else {
           o.x = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
           o.y = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
@@ -253,7 +280,7 @@ __global__ void __launch_bounds__(256, NCH <= 5 ? 4 : 2) rms_norm_quant_kernel(c
       for (int e = 0; e < 8; ++e) {
         if (at(i, e) >= a.D) continue;
         uint32_t code = 0;
-        if constexpr (E4M3) code = detail::code_e4m3x2(v[i][e], 0.0f);
+        if constexpr (E4M3) code = up[e / 4] >> (8 * (e % 4));
         else code = c[e];
         if (row_ok) q[at(i, e)] = static_cast<uint8_t>(good ? code : 0u);
       }
@@ -283,7 +310,7 @@ __global__ void __launch_bounds__(256, NCH <= 5 ? 4 : 2) rms_norm_quant_kernel(c
         const int k = 32 * m + __ffs(left) - 1, c = at(k >> 3, k & 7);
         if (c >= a.D) continue;
         const double num = product64(c) * 448.0;
-        if (fabs(num) >= 0.015625 * den && fabs(num) < 448.0 * den)  // from 2^-6 on steps are relative: e4m3's normal range
+        if (fabs(num) < 448.0 * den)
           q[c] = static_cast<uint8_t>(detail::code_e4m3x2(detail::nearest_e4m3(num, den), 0.0f));
       }
   }

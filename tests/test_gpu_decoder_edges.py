@@ -39,6 +39,27 @@ def test_rms_norm_quant_e4m3_short_rows_share_a_block(d, dtype):
     assert torch.equal(codes.double()[normal], _nearest_e4m3(t)[normal])
 
 
+@pytest.mark.parametrize("dtype, d", [(F32, 1536), (F32, 200), (F32, 777), (BF, 5120)])
+def test_rms_norm_quant_e4m3_small_quotients_are_exact_too(dtype, d):
+    """Rows with a few channels far larger than the rest have most of their quotients below 2^-6, where e4m3's steps are
+    absolute: tens of millions of values, none on the wrong side of a border."""
+    from dsaquant_b200.kernels.rms_norm import rms_norm_quant
+
+    g = _gen(52 + d)
+    w = 0.5 + torch.rand(d, generator=g, device="cuda")
+    w[::97] *= 50000.0
+    w = w.to(dtype)
+    small = 0
+    for _ in range(10):
+        x = _randn(g, 4_000_000 // d, d, dtype=dtype)
+        codes, _ = rms_norm_quant(x, w, out_dtype=torch.float8_e4m3fn)
+        y = x.double() * w.double()
+        t = y * 448 / y.abs().amax(-1, keepdim=True)
+        assert torch.equal(codes.double(), _nearest_e4m3(t))
+        small += int((t.abs() < 2.0 ** -6).sum())
+    assert small > 10_000_000
+
+
 def test_rms_norm_quant_e4m3_largest_value_in_64_bits():
     """Two values so close that their fp32 products come out in the wrong order, and quotients that lie on one side of a
     border for one of them and on the other side for the other.  Rows of whole numbers, whose squares add up exactly."""
