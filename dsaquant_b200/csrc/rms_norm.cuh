@@ -16,7 +16,9 @@
 // two products, the same for the largest value, scale, reciprocal, product: ten halves of 2^-23) are less.  A value with two
 // codes (one in 2^15) is read again and decided in 64 bits, against the
 // row's largest |s * weight|, of which 64 bits are kept too; the rsqrt cancels.  The largest is sought among all values
-// within 2^-20 of the fp32 maximum, whose order three roundings each may have changed (2^-21.4).
+// within 2^-20 of the fp32 maximum, whose order three roundings each may have changed (2^-21.4).  In a row whose scale is the
+// least one (max|y| <= 1e-5, or so near that 64 bits have to tell) the rsqrt does not cancel: it is computed again in 64
+// bits, by each thread that needs it, and the nudges are 2^-18, for the sum of squares is off by up to 77 halves of 2^-23.
 //
 // A row whose sum of squares or whose y is not finite has no meaningful codes: its scale is NaN
 // (whatever is computed from it shows it) and its codes are 0.
@@ -224,13 +226,14 @@ __global__ void __launch_bounds__(256, NCH <= 5 ? 4 : 2) rms_norm_quant_kernel(c
   if (!(amax < INFINITY)) amax = INFINITY;
   amax = row_reduce<TPR, true>(amax, red[1], sub);
   const bool good = ss < INFINITY && amax < INFINITY;  // false for NaN
+  [[maybe_unused]] const bool least = amax < 1.0001e-5f;
   const float top = E4M3 ? 448.0f : 127.0f;
   const float s = __fmul_rn(__fdiv_rn(fmaxf(amax, 1e-5f), top), a.clip);
   [[maybe_unused]] float inv_up = 0.0f, inv_dn = 0.0f;
   if constexpr (E4M3) {
-    const float inv = __fdiv_rn(1.0f, s);
-    inv_up = inv * 1.00000095f;  // 1 + 2^-20
-    inv_dn = inv * 0.99999905f;
+    const float inv = __fdiv_rn(1.0f, s), nudge = least ? 3.8146973e-06f : 9.5367432e-07f;  // 2^-18, 2^-20
+    inv_up = inv * (1.0f + nudge);
+    inv_dn = inv * (1.0f - nudge);
   }
   [[maybe_unused]] const detail::RowQuant rq = detail::row_quant_of<127>(s, a.clip);
   uint8_t* q = static_cast<uint8_t*>(a.codes) + (row_ok ? row : 0) * a.D;
@@ -287,14 +290,17 @@ __global__ void __launch_bounds__(256, NCH <= 5 ? 4 : 2) rms_norm_quant_kernel(c
     }
   }
   if constexpr (E4M3) {
-    auto product64 = [&](int c) {  // s * weight of one value, read again
-      double s64 = static_cast<double>(detail::load_f32(xr + c));
-      if (rr != nullptr) s64 += static_cast<double>(detail::load_f32(rr + c));
+    auto sum64 = [&](int c) {  // one value of s, read again
+      const double s64 = static_cast<double>(detail::load_f32(xr + c));
+      return rr != nullptr ? s64 + static_cast<double>(detail::load_f32(rr + c)) : s64;
+    };
+    auto product64 = [&](int c) {  // s * weight
+      const double s64 = sum64(c);
       if (a.w_dtype == XDT_F16) return s64 * static_cast<double>(detail::load_f32(static_cast<const __half*>(a.weight) + c));
       if (a.w_dtype == XDT_BF16) return s64 * static_cast<double>(detail::load_f32(static_cast<const __nv_bfloat16*>(a.weight) + c));
       return s64 * static_cast<double>(detail::load_f32(static_cast<const float*>(a.weight) + c));
     };
-    const bool decide = row_ok && good && amax > 1e-5f;
+    const bool decide = row_ok && good;
 #pragma unroll
     for (int m = 0; m < MW; ++m)
       for (uint32_t left = decide ? largest[m] : 0u; left != 0; left &= left - 1) {
@@ -303,7 +309,15 @@ __global__ void __launch_bounds__(256, NCH <= 5 ? 4 : 2) rms_norm_quant_kernel(c
           atomicMax(&top64[sub], static_cast<unsigned long long>(__double_as_longlong(fabs(product64(c)))));
       }
     __syncthreads();
-    const double den = __longlong_as_double(static_cast<long long>(top64[sub])) * static_cast<double>(a.clip);
+    double den = __longlong_as_double(static_cast<long long>(top64[sub])) * static_cast<double>(a.clip);
+    uint32_t any = 0;
+#pragma unroll
+    for (int m = 0; m < MW; ++m) any |= near[m];
+    if (decide && least && any != 0) {  // |y| <= 1e-5 in the units of |s * weight|
+      double ss64 = 0.0;
+      for (int c = 0; c < a.D; ++c) ss64 = fma(sum64(c), sum64(c), ss64);
+      den = fmax(den, 1e-5 * static_cast<double>(a.clip) * sqrt(ss64 / a.D + static_cast<double>(a.eps)));
+    }
 #pragma unroll
     for (int m = 0; m < MW; ++m)
       for (uint32_t left = decide ? near[m] : 0u; left != 0; left &= left - 1) {

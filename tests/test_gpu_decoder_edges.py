@@ -92,6 +92,26 @@ def test_rms_norm_quant_e4m3_largest_value_in_64_bits():
     assert found > 10
 
 
+@pytest.mark.parametrize("d, eps", [(1536, 1.0), (200, 0.25), (777, 1.0), (64, 2.0 ** -10)])
+def test_rms_norm_quant_e4m3_rows_with_the_least_scale_are_exact_too(d, eps):
+    """Rows of max|y| up to and around 1e-5, whose scale does not follow them."""
+    from dsaquant_b200.kernels.rms_norm import rms_norm_quant
+
+    g = _gen(54 + d)
+    w = 1 + 0.1 * _randn(g, d)
+    least = 0
+    for _ in range(6):
+        m = 3_000_000 // d
+        x = (2 * torch.rand(m, d, generator=g, device="cuda") - 1) * eps ** 0.5 * 1e-5
+        x[::3] *= torch.rand(len(x[::3]), 1, generator=g, device="cuda")
+        codes, scale = rms_norm_quant(x, w, eps, out_dtype=torch.float8_e4m3fn)
+        y = x.double() * w.double() * torch.rsqrt(x.double().square().mean(-1, keepdim=True) + eps)
+        top = y.abs().amax(-1, keepdim=True)
+        assert torch.equal(codes.double(), _nearest_e4m3(y * 448 / top.clamp_min(1e-5)))
+        least += int((top < 1e-5).sum())
+    assert least > 1000
+
+
 @pytest.mark.parametrize("d, clip", [(512, 1.0), (5120, 1.0), (777, 0.9), (64, 0.5)])
 def test_rms_norm_quant_int8_codes_are_those_of_the_division(d, clip):
     """codes = clamp(rint(y / scale)) with fp32's quotient, as the package's other quantiser rounds, at quotients beside the
