@@ -21,7 +21,8 @@
 // bits, by each thread that needs it, and the nudges are 2^-18, for the sum of squares is off by up to 77 halves of 2^-23.
 //
 // A row whose sum of squares or whose y is not finite has no meaningful codes: its scale is NaN
-// (whatever is computed from it shows it) and its codes are 0.
+// (whatever is computed from it shows it) and its codes are 0.  So it is for a row whose mean square and eps add up to less
+// than the least normal number (squares below it have lost bits, or are 0), and for a scale without a normal reciprocal.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -198,7 +199,8 @@ __global__ void __launch_bounds__(256, NCH <= 5 ? 4 : 2) rms_norm_quant_kernel(c
 #pragma unroll
     for (int e = 0; e < 8; ++e) ss = fmaf(v[i][e], v[i][e], ss);
   ss = row_reduce<TPR, false>(ss, red[0], sub);
-  const float rstd = rsqrtf(ss / static_cast<float>(a.D) + a.eps);
+  const float mean = ss / static_cast<float>(a.D) + a.eps;
+  const float rstd = rsqrtf(mean);
 
   float amax = 0.0f;
   auto normalise = [&](const auto* weight) {
@@ -225,10 +227,11 @@ __global__ void __launch_bounds__(256, NCH <= 5 ? 4 : 2) rms_norm_quant_kernel(c
   // a NaN must survive the reduction too: it travels as +inf, which no finite row reaches
   if (!(amax < INFINITY)) amax = INFINITY;
   amax = row_reduce<TPR, true>(amax, red[1], sub);
-  const bool good = ss < INFINITY && amax < INFINITY;  // false for NaN
   [[maybe_unused]] const bool least = amax < 1.0001e-5f;
   const float top = E4M3 ? 448.0f : 127.0f;
   const float s = __fmul_rn(__fdiv_rn(fmaxf(amax, 1e-5f), top), a.clip);
+  constexpr float kLeast = 1.17549435e-38f, kMost = 8.5070592e37f;  // 2^-126, 2^126
+  const bool good = ss < INFINITY && amax < INFINITY && (mean >= kLeast || amax == 0.0f) && s >= kLeast && s <= kMost;  // false for NaN
   [[maybe_unused]] float inv_up = 0.0f, inv_dn = 0.0f;
   if constexpr (E4M3) {
     const float inv = __fdiv_rn(1.0f, s), nudge = least ? 3.8146973e-06f : 9.5367432e-07f;  // 2^-18, 2^-20

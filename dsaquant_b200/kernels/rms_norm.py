@@ -41,7 +41,8 @@ def rms_norm_quant(
 
     Everything is fp32 and reads s before its rounding.  D is at most 16384.  Rows may be strided (views of a
     wider tensor are read in place).  A row whose sum of squares is not finite in fp32 (it
-    holds an infinity, a NaN, or values near 1e19) has scale NaN and codes 0.  Forward only, as every operator here."""
+    holds an infinity, a NaN, or values near 1e19), whose mean square and eps add up to less than fp32's normal range (values
+    below 1e-19 with an eps of 0), or whose scale leaves 1.2e-38 .. 8.5e37 has scale NaN and codes 0.  Forward only, as every operator here."""
     lib = _load_ext()
     _require_cuda(x, "x")
     if x.dtype not in _DTYPE_CODE or weight.dtype not in _DTYPE_CODE:

@@ -28,7 +28,8 @@ extern "C" {
  * residual and residual_out are both given or both NULL.  The arithmetic is fp32 and reads s before its
  * rounding; e4m3 codes are decided in 64 bits where fp32 cannot tell two neighbours apart.  1 <= D <= 16384.
  * int8 codes and scales are what b200w4a4_gemm and b200w4a4_linear_w4_group take.
- * A row that is not finite gets scale NaN and codes 0. */
+ * A row that is not finite, whose mean(s^2) + eps is below fp32's normal range (and not a row of zeros with
+ * eps > 0), or whose scale has no normal reciprocal gets scale NaN and codes 0. */
 int b200w4a4_rms_norm_quant(const void* x, int x_dtype, long long x_ld, const void* residual,
                             long long residual_ld, const void* weight, int w_dtype, float eps,
                             void* codes, int code_format, float* scale, void* residual_out, int M,

@@ -133,6 +133,35 @@ def test_rms_norm_quant_int8_codes_are_those_of_the_division(d, clip):
     assert torch.equal(codes.float(), (x / scale).round().clamp(-128, 127))
 
 
+@pytest.mark.parametrize("out_dtype", [torch.int8, torch.float8_e4m3fn])
+def test_rms_norm_quant_rows_outside_the_range_of_fp32_are_marked(out_dtype):
+    """Squares that leave fp32's normal range, and scales whose reciprocal does, give NaN and codes 0, not numbers that are off."""
+    from dsaquant_b200.kernels.rms_norm import rms_norm_quant
+
+    g = _gen(57)
+    x = _randn(g, 8, 300)
+    x[1] *= 1e-17
+    x[2] *= 1e-22
+    x[3] *= 1e-30
+    x[4] = 0
+    w = 1 + 0.1 * _randn(g, 300)
+    top = 127.0 if out_dtype == torch.int8 else 448.0
+    y = x.double() * torch.rsqrt(x.double().square().mean(-1, keepdim=True)) * w.double()
+    want = y.abs().amax(-1) / top
+    codes, scale = rms_norm_quant(x, w, 0.0, out_dtype=out_dtype)
+    fine = [0, 1, 5, 6, 7]
+    # as in _check_rms: 300 squares in a row's 32 threads, then the root, two products and a quotient
+    _within(scale[fine], want[fine], (74 / 2 + 8) * 2.0 ** -24 * want[fine])
+    assert bool(torch.isnan(scale[[2, 3, 4]]).all()) and bool((codes[[2, 3, 4]].float() == 0).all())
+    codes, scale = rms_norm_quant(x, w, 1e-30, out_dtype=out_dtype)   # an eps of any use keeps them
+    assert bool(torch.isfinite(scale).all()) and bool((codes[4].float() == 0).all())
+    for clip, marked in ((1e-34, True), (1e-25, False), (1e25, False)):
+        codes, scale = rms_norm_quant(x[4:6], w, out_dtype=out_dtype, clip_ratio=clip)
+        # of the row of zeros, whose scale is 1e-5 / top * clip
+        assert bool(torch.isnan(scale[0])) == marked and bool((codes[0].float() == 0).all())
+        assert bool(torch.isfinite(scale[1]))
+
+
 # ------------------------------------------------------------------------------------------------ window_attention
 def _attention_bound(q, k, v, window, sinks, lens):
     """The definition in 64 bits and how far a result may be off (the terms are explained at _check_attention)."""
