@@ -303,14 +303,15 @@ __global__ void __launch_bounds__(256, NCH <= 5 ? 4 : 2) rms_norm_quant_kernel(c
       if (a.w_dtype == XDT_BF16) return s64 * static_cast<double>(detail::load_f32(static_cast<const __nv_bfloat16*>(a.weight) + c));
       return s64 * static_cast<double>(detail::load_f32(static_cast<const float*>(a.weight) + c));
     };
-    const bool decide = row_ok && good;
+    const bool decide = row_ok && good && amax > 0.0f;  // in a row of zeros every value is the largest
+    unsigned long long mine = 0;  // positive 64-bit floats order as integers
 #pragma unroll
     for (int m = 0; m < MW; ++m)
       for (uint32_t left = decide ? largest[m] : 0u; left != 0; left &= left - 1) {
         const int k = 32 * m + __ffs(left) - 1, c = at(k >> 3, k & 7);
-        if (c < a.D)  // positive 64-bit floats order as integers
-          atomicMax(&top64[sub], static_cast<unsigned long long>(__double_as_longlong(fabs(product64(c)))));
+        if (c < a.D) mine = max(mine, static_cast<unsigned long long>(__double_as_longlong(fabs(product64(c)))));
       }
+    if (mine != 0) atomicMax(&top64[sub], mine);
     __syncthreads();
     double den = __longlong_as_double(static_cast<long long>(top64[sub])) * static_cast<double>(a.clip);
     uint32_t any = 0;
