@@ -636,8 +636,11 @@ __global__ void __launch_bounds__(128) window_attn_join_kernel(const WindowAttnA
 // 16 rows reads the keys again, from L2), more the one with 64-row tiles.
 inline bool window_attn_decodes(long long rows) { return rows <= 2 * kAttnDecodeRows; }
 
-// Runs the keys of a row tile are split into: enough for four CTAs an SM, none longer than 1024 keys (sequences of
-// unequal lengths share the GPU evenly then), none shorter than two key tiles.
+// Runs the keys of a row tile are split into: enough for four CTAs an SM, none shorter than two key tiles, at most 64 (and at
+// most 65535 / B, see attention_splits).  The single-token kernel's are also no longer than 1024 keys while that allows it, so
+// that sequences of unequal lengths share the GPU evenly; its partial outputs, 32 rows a key head at most, are then a
+// thirtieth of the keys and values.  In the 64-row form they would be an eighth for every tile of rows (1.3 GB for 32 x 127
+// queries of 40 heads of 128 on 16000 keys, for 42 MB of output), so there the first rule alone counts.
 inline int window_attn_splits(int B, int Lq, int Lk, int Hkv, int G, int window, int sinks, int sm_count) {
   const long long rows = static_cast<long long>(Lq) * G;
   const int per_tile = window_attn_decodes(rows) ? kAttnDecodeRows : kAttnRows;
@@ -647,7 +650,7 @@ inline int window_attn_splits(int B, int Lq, int Lk, int Hkv, int G, int window,
   const long long keys = Lk < reach ? Lk : (Lk < reach + sinks ? Lk : reach + sinks);
   const long long key_tiles = (keys + kAttnBN - 1) / kAttnBN + 1;  // a window need not start at a tile's edge
   long long s = (4LL * sm_count + tiles - 1) / tiles;
-  if (s < (key_tiles + 15) / 16) s = (key_tiles + 15) / 16;
+  if (window_attn_decodes(rows) && s < (key_tiles + 15) / 16) s = (key_tiles + 15) / 16;
   if (s > key_tiles / 2) s = key_tiles / 2;
   if (s > 64) s = 64;
   return s < 1 ? 1 : static_cast<int>(s);

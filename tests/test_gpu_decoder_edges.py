@@ -227,6 +227,28 @@ def test_window_attention_every_value_not_finite():
     assert vdm.last_device_status() == 0
 
 
+@pytest.mark.parametrize("b, lq, lk, hq, hk, hd", [
+    (32, 127, 16000, 40, 8, 128), (32, 127, 65536, 40, 8, 128), (1, 127, 65536, 8, 8, 128), (4, 33, 8000, 4, 4, 64), (64, 64, 4000, 16, 1, 128),
+    (16, 1, 8192, 40, 8, 128), (1, 1, 500000, 64, 1, 128), (64, 2, 100000, 16, 1, 64)])
+def test_window_attention_workspace_stays_small(b, lq, lk, hq, hk, hd):
+    """Partial outputs are a small part of the keys and values, or what four blocks an SM hold twice over."""
+    from dsaquant_b200 import _lib
+
+    need = _lib.load().b200w4a4_window_attention_workspace_bytes(b, lq, lk, hq, hk, hd, lk, 0)
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    few = 2 * 4 * sms * 64 * (hd + 1) * 4
+    assert need <= max(few, 4 * b * lk * hk * hd // 16)
+
+
+def test_window_attention_prompts_need_no_workspace():
+    """The wrapper asks for none from PROMPT_QUERIES queries on, and the library wants none from there on."""
+    from dsaquant_b200 import _lib
+    from dsaquant_b200.window_attention import PROMPT_QUERIES
+
+    need = _lib.load().b200w4a4_window_attention_workspace_bytes
+    assert need(1, PROMPT_QUERIES, 100000, 8, 8, 128, 100000, 0) == 0 and need(1, PROMPT_QUERIES - 1, 100000, 8, 8, 128, 100000, 0) > 0
+
+
 # ------------------------------------------------------------------------------------------------ apply_rotary
 def test_apply_rotary_inplace_refuses_shared_memory():
     """q and k that overlap each other, or tokens that overlap, would be rotated twice; out of place they are read only."""
