@@ -56,6 +56,9 @@ def rotary_table(
 
         low, high = max(math.floor(pair_of(beta_fast)), 0), min(math.ceil(pair_of(beta_slow)), rotary_dim - 1)
         ramp = ((i - low) / max(high - low, 0.001)).clamp(0, 1)
+        # where the clamps moved an end of the ramp (a short trained length, a slow base): no pair on its wrong side
+        turns = trained_positions * f / (2 * math.pi)
+        ramp = torch.where(turns < beta_slow, 1.0, torch.where(turns > beta_fast, 0.0, ramp))
         f = f * (1 - ramp) + f / factor * ramp
         amplitude = 0.1 * math.log(factor) + 1.0
     angle = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] * f

@@ -233,3 +233,42 @@ def test_weights_in_the_gemms_order_are_known_as_such(tmp_path):
 @pytest.mark.parametrize("over, code", [(dict(odt=16, bias=P + 2), -3), (dict(odt=18), -1), (dict(odt=17, m=0), 0), (dict(odt=32), -1)])
 def test_linear_w4_group_fp32_bias_refusals(lib, over, code):
     assert _w4(lib, **over) == code
+
+
+@pytest.mark.parametrize("trained, base, rd", [(4, 10000.0, 64), (6, 10000.0, 64), (1, 10000.0, 32), (4096, 2.0, 16), (1 << 20, 1.5, 8), (4096, 10000.0, 128),
+                                               (131072, 500000.0, 128)])
+def test_yarn_tables_keep_fast_pairs_and_stretch_slow_ones(trained, base, rd):
+    """Every pair against the two sentences of the definition, where the trained length or the base leaves no room for a ramp too;
+    between them, the angles lie between the two."""
+    from dsaquant_b200.rotary import rotary_table
+
+    factor, positions = 8.0, 50
+    table = rotary_table(positions, rd, base, scaling="yarn", factor=factor, trained_positions=trained).double() / (0.1 * math.log(factor) + 1)
+    p = torch.arange(positions, dtype=torch.float64)
+    for i in range(rd // 2):
+        f = base ** (-2 * i / rd)
+        turns = trained * f / (2 * math.pi)
+        # two roundings to fp32, of the table and of what it was divided by
+        same = lambda a: bool(((table[:, i, 0] - (p * a).cos()).abs() < 2.0 ** -22).all() and ((table[:, i, 1] - (p * a).sin()).abs() < 2.0 ** -22).all())  # noqa: E731
+        if turns > 32:
+            assert same(f)
+        elif turns < 1:
+            assert same(f / factor)
+        else:
+            angle = math.atan2(table[1, i, 1], table[1, i, 0])
+            assert f / factor - 1e-6 <= angle <= f + 1e-6
+
+
+def test_yarn_ramp_is_linear_in_the_pair():
+    """The usual sizes: between the pair that turns 32 times over the trained length and the one that turns once."""
+    from dsaquant_b200.rotary import rotary_table
+
+    rd, base, factor, trained = 128, 10000.0, 8.0, 4096
+    table = rotary_table(2, rd, base, scaling="yarn", factor=factor, trained_positions=trained).double()
+    low = math.floor(rd * math.log(trained / (32 * 2 * math.pi)) / (2 * math.log(base)))
+    high = math.ceil(rd * math.log(trained / (2 * math.pi)) / (2 * math.log(base)))
+    assert (low, high) == (20, 46)
+    for i in range(rd // 2):
+        f, ramp = base ** (-2 * i / rd), min(max((i - low) / (high - low), 0.0), 1.0)
+        want = f * (1 - ramp) + f / factor * ramp
+        assert abs(math.atan2(table[1, i, 1], table[1, i, 0]) - want) < 2.0 ** -22
