@@ -386,11 +386,13 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
       }
       // Weights against the maximum known so far.  A row that has none yet, or whose weights of this tile add up to
       // over 2^9 in one half (the only sign that the maximum moved far), makes its warps find the maximum and do
-      // them again.  Only such a row's maximum moves, so what a row gets does not depend on the rows beside it.
+      // them again.  Only such a row's maximum moves, so what a row gets does not depend on the rows beside it.  One more
+      // turn is always enough - a row that has found its maximum here has weights of at most 1, the others' sums stay as they
+      // were - and the loop ends there whatever the scores are: sums that are not finite would ask for ever.
       float sum;
       bool mine = m == -INFINITY, find = __any_sync(0xffffffffu, mine);  // the same for both halves
 #pragma unroll 1
-      while (true) {
+      for (int turn = 0;; ++turn) {
         if (find) {
           float top = __uint_as_float(s[0]);  // a NaN score makes it NaN
 #pragma unroll
@@ -445,6 +447,7 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         float sum1;
         unpair(both, sum, sum1);
         sum += sum1;
+        if (turn > 0) break;
         const bool bad = !mine && !(sum <= 512.0f);  // a row that just moved has weights of at most 1
         find = meet_any(bad);
         if (!find) break;

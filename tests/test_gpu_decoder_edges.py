@@ -227,6 +227,42 @@ def test_window_attention_every_value_not_finite():
     assert vdm.last_device_status() == 0
 
 
+@pytest.mark.parametrize("dtype, hd", [(BF, 128), (FP, 64)])
+@pytest.mark.parametrize("lq, lk, window, sinks", [(400, 400, 90, 0), (300, 900, 200, 0), (256, 256, 64, 0), (500, 500, 90, 3), (300, 300, 5000, 0),
+                                                   (60, 400, 90, 0), (3, 400, 90, 0)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_window_attention_not_finite_rows_and_keys_without_first_keys(lq, lk, window, sinks, dtype, hd, value):
+    """Rows of a block whose windows begin in different key tiles, all with scores that are not finite - one bad key that they
+    share, or queries that hold garbage - end, give NaN where the definition does, and leave the other rows as they are."""
+    from dsaquant_b200.kernels import vdm_w4a4 as vdm
+    from dsaquant_b200.window_attention import window_attention
+
+    g = _gen(63 + lq + window)
+    q, k, v = _qkv(g, 2, lq, lk, 2, 1, hd, dtype)
+    q[..., 0] = q[..., 0].abs() + 1                                   # an infinite key scores with the sign it has
+    lens = torch.tensor([lk, lk - 40], dtype=torch.int32, device="cuda")
+    clean, clean_lse = window_attention(q, k, v, window, sinks, kv_lens=lens, return_lse=True)
+    at = lens.long()[:, None] - lq + torch.arange(lq, device="cuda")
+    for key in (lk - 41, lk - 100, lk - 129, lk - 200, max(lk - lq, 0)):
+        bad = k.clone()
+        bad[:, key, :, 0] = value
+        out, lse = window_attention(q, bad, v, window, sinks, kv_lens=lens, return_lse=True)
+        sees = (at >= key) & ((at < key + window) | (key < sinks))
+        assert torch.equal(out[~sees], clean[~sees])
+        assert torch.equal(lse.transpose(1, 2)[~sees], clean_lse.transpose(1, 2)[~sees])
+        if value != float("-inf"):                                    # (a score of -inf is a weight of 0)
+            assert bool(torch.isnan(out[sees]).all()) and not bool(torch.isfinite(lse.transpose(1, 2)[sees]).any())
+    some = torch.zeros(2, lq, dtype=torch.bool, device="cuda")
+    some[:, ::2] = some[:, lq // 2:lq // 2 + 40] = True
+    bad = q.clone()
+    bad[some] = value                                                 # whole queries: scores of both signs, or NaN
+    out, lse = window_attention(bad, k, v, window, sinks, kv_lens=lens, return_lse=True)
+    none = at < 0
+    assert torch.equal(out[~some], clean[~some]) and bool((out[none] == 0).all())
+    assert not bool(torch.isfinite(lse.transpose(1, 2)[some & ~none]).any())
+    assert vdm.last_device_status() == 0
+
+
 @pytest.mark.parametrize("b, lq, lk, hq, hk, hd", [
     (32, 127, 16000, 40, 8, 128), (32, 127, 65536, 40, 8, 128), (1, 127, 65536, 8, 8, 128), (4, 33, 8000, 4, 4, 64), (64, 64, 4000, 16, 1, 128),
     (16, 1, 8192, 40, 8, 128), (1, 1, 500000, 64, 1, 128), (64, 2, 100000, 16, 1, 64)])
