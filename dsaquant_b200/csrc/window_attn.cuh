@@ -10,9 +10,9 @@
 // those are visited; the mask is evaluated only in tiles that some row does not see entirely.
 // Keys that no row of the tile sees are read as zeros, so whatever lies there (freed or unwritten cache
 // lines, NaN among them) has no effect.  A key that some rows of the tile see and others do not enters the second
-// product of all of them, of the others with weight 0 - and 0 * inf is NaN.  A row whose sum of weights is finite
-// and whose output is not is therefore computed again from its own keys alone (row_by_definition), at the end and by the
-// warp that has it: V that is finite costs one test a value, and nothing in the loops.
+// product of all of them, of the others with weight 0 - and 0 * inf is NaN.  So in the key tiles that some row does not see
+// entirely, values of V that are not finite are replaced by zeros in shared memory, and only if there were any, the rows that
+// see them get them added at the end: their sum is then inf or NaN as by the formula, whatever the finite rest is.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -118,48 +118,50 @@ __device__ __forceinline__ int swz(int r, int c) {
   return r * HD + ((c ^ (r & 7)) << 3);
 }
 
-// W columns from c0 on of the output of query qi, head qh, over the keys that the row sees in the key tiles
-// [first, last) of BN keys: sum_j exp2(q . k_j * scale * log2(e) - lse2) v_j in fp32, lse2 the row's log-sum-exp (in units of
-// log2, finite) over these keys.  All lanes of a warp take part: each scores one of 32 keys, then each adds up its columns.
-template <typename T, int HD, int W, int BN, typename Out>
-__device__ __noinline__ void row_by_definition(const WindowAttnArgs& a, const Span& sp, int b, int qi, int qh, int first,
-                                               int last, float lse2, int c0, Out* out) {
-  const int lane = threadIdx.x & 31;
-  int len = a.Lk;
-  if (a.kv_lens != nullptr) len = min(max(a.kv_lens[b], 0), a.Lk);
-  const int p = len - a.Lq + qi, hk = qh / a.G;
-  const T* q = static_cast<const T*>(a.q) + b * a.q_b + qi * a.q_t + qh * a.q_h;
-  const T* kb = static_cast<const T*>(a.k) + b * a.k_b + hk * a.k_h;
-  const T* vb = static_cast<const T*>(a.v) + b * a.v_b + hk * a.v_h + c0 + lane;
-  const float sc = a.scale * kLog2e;
-  float acc[W / 32] = {};
-  for (int n = first; n < last; ++n)
-    for (int half = 0; half < BN; half += 32) {
-      const int j0 = (n < sp.n_sink ? n : sp.w0 + n - sp.n_sink) * BN + half, j = j0 + lane;
-      const bool sees = j <= p && (j > p - a.window || j < a.sinks);
-      float w = 0.0f;
-      if (sees) {
-        const T* k = kb + j * a.k_t;
-        float s = 0.0f;
-        for (int c = 0; c < HD; c += 8) {
-          const uint4 x = __ldg(reinterpret_cast<const uint4*>(q + c)), y = __ldg(reinterpret_cast<const uint4*>(k + c));
-          const T* xt = reinterpret_cast<const T*>(&x);
-          const T* yt = reinterpret_cast<const T*>(&y);
+// Bit 15 of each 16-bit half that is an infinity or a NaN.
+__device__ __forceinline__ uint32_t not_finite(uint32_t w, __half) { return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u; }
+__device__ __forceinline__ uint32_t not_finite(uint32_t w, __nv_bfloat16) { return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
+
+template <typename T>
+__device__ __forceinline__ bool any_not_finite(const void* p) {
+  const uint4 v = *static_cast<const uint4*>(p);
+  return (not_finite(v.x, T()) | not_finite(v.y, T()) | not_finite(v.z, T()) | not_finite(v.w, T())) != 0;
+}
+
+// Eight values in shared memory: those that are not finite become 0.  True if there were any.
+template <typename T>
+__device__ __forceinline__ bool clear_not_finite(void* p) {
+  uint4 v = *static_cast<const uint4*>(p);
+  const uint32_t x = not_finite(v.x, T()), y = not_finite(v.y, T()), z = not_finite(v.z, T()), w = not_finite(v.w, T());
+  if ((x | y | z | w) == 0) return false;
+  v.x &= ~((x >> 15) * 0xffffu);
+  v.y &= ~((y >> 15) * 0xffffu);
+  v.z &= ~((z >> 15) * 0xffffu);
+  v.w &= ~((w >> 15) * 0xffffu);
+  *static_cast<uint4*>(p) = v;
+  return true;
+}
+
+// Adds the values that are not finite of V's keys [j0, j0 + KEYS) to a thread's two rows (columns 8 h + 2 t and the next) that see them.
+template <typename T, int HD, int KEYS>
+__device__ __forceinline__ void add_not_finite(float (&o)[HD / 8][4], const T* v, long long v_t, int j0, const int (&pos)[2],
+                                               int window, int sinks) {
+#pragma unroll 1
+  for (int j = j0; j < j0 + KEYS; ++j) {
+    bool sees[2];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) s = fmaf(static_cast<float>(xt[i]), static_cast<float>(yt[i]), s);
-        }
-        w = exp2_fast(fmaf(s, sc, -lse2));
-      }
-      for (unsigned left = __ballot_sync(0xffffffffu, sees); left != 0; left &= left - 1) {
-        const int l = __ffs(left) - 1;
-        const float wl = __shfl_sync(0xffffffffu, w, l);
-        const T* v = vb + (j0 + l) * a.v_t;
+    for (int i = 0; i < 2; ++i) sees[i] = j <= pos[i] && (j > pos[i] - window || j < sinks);
+    if (!sees[0] && !sees[1]) continue;
+    const uint32_t* row = reinterpret_cast<const uint32_t*>(v + j * v_t);
 #pragma unroll
-        for (int i = 0; i < W / 32; ++i) acc[i] = fmaf(wl, static_cast<float>(v[32 * i]), acc[i]);
-      }
+    for (int h = 0; h < HD / 8; ++h) {
+      const uint32_t w = __ldg(row + 4 * h), bad = not_finite(w, T());
+      const T* x = reinterpret_cast<const T*>(&w);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (sees[k >> 1] && (bad >> (16 * (k & 1) + 15) & 1) != 0) o[h][k] += static_cast<float>(x[k & 1]);
     }
-#pragma unroll
-  for (int i = 0; i < W / 32; ++i) out[lane + 32 * i] = static_cast<Out>(acc[i]);
+  }
 }
 
 }  // namespace attn
@@ -169,7 +171,7 @@ __device__ __noinline__ void row_by_definition(const WindowAttnArgs& a, const Sp
 constexpr int kAttnRows = 64, kAttnBN = 64;
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(128) window_attn_kernel(const __grid_constant__ WindowAttnArgs a) {
+__global__ void __launch_bounds__(128) window_attn_kernel(const WindowAttnArgs a) {
   using namespace attn;
   constexpr int BN = kAttnBN, KT = HD / 16;
   extern __shared__ __align__(128) uint8_t smem_raw[];
@@ -236,13 +238,26 @@ __global__ void __launch_bounds__(128) window_attn_kernel(const __grid_constant_
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
   const float sc = a.scale * kLog2e;
 
+  // every row sees the whole tile when its last key is at or before the first position and its first
+  // key is inside the last position's window
+  auto sees_all = [&](int j0) { return j0 + BN - 1 <= sp.p0 && (j0 > sp.p1 - a.window || j0 + BN <= a.sinks); };
+  bool cleared = false;  // of V, somewhere
   if (first < last) load(first, 0);
   cp_commit();
   for (int n = first; n < last; ++n) {
     const int stage = (n - first) & 1;
+    const int j0 = tile_key(n);
+    const bool whole = sees_all(j0);
     if (n + 1 < last) load(n + 1, stage ^ 1);
     cp_commit();
     cp_wait<1>();
+    if (!whole && sp.p0 != sp.p1) {  // (rows of one position see the same keys)
+#pragma unroll
+      for (int i = 0; i < BN * (HD / 8) / 128; ++i) {  // the chunks that this thread copied
+        const int c = threadIdx.x + i * 128;
+        cleared |= clear_not_finite<T>(sv + stage * BN * HD + swz<HD>(c / (HD / 8), c % (HD / 8)));
+      }
+    }
     __syncthreads();
     const T* ks = sk + stage * BN * HD;
     const T* vs = sv + stage * BN * HD;
@@ -262,10 +277,6 @@ __global__ void __launch_bounds__(128) window_attn_kernel(const __grid_constant_
         mma(s[2 * nt + 1], qf[kt], f[2], f[3], T());
       }
     }
-    const int j0 = tile_key(n);
-    // every row sees the whole tile when its last key is at or before the first position and its first
-    // key is inside the last position's window
-    const bool whole = j0 + BN - 1 <= sp.p0 && (j0 > sp.p1 - a.window || j0 + BN <= a.sinks);
     if (!whole) {
 #pragma unroll
       for (int i = 0; i < BN / 8; ++i)
@@ -318,49 +329,29 @@ __global__ void __launch_bounds__(128) window_attn_kernel(const __grid_constant_
     __syncthreads();
   }
 
+  if (__syncthreads_or(cleared))
+    for (int n = first; n < last; ++n)
+      if (!sees_all(tile_key(n))) add_not_finite<T, HD, BN>(o, vb + 2 * t, a.v_t, tile_key(n), pos, a.window, a.sinks);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    if (!row_ok[i]) continue;
     const float inv = l[i] > 0.0f ? 1.0f / l[i] : (l[i] == 0.0f ? 0.0f : l[i]);
     const float lse2 = l[i] == 0.0f ? -INFINITY : m[i] + log2f(l[i]);
     const long long head_row = (static_cast<long long>(b) * a.Hq + qh[i]) * a.Lq + qi[i];
-    const long long at = static_cast<long long>(split) * a.B * a.Hq * a.Lq + head_row;
-    T* out = static_cast<T*>(a.out) + ((static_cast<long long>(b) * a.Lq + qi[i]) * a.Hq + qh[i]) * HD;
-    float finite = 0.0f;  // NaN once a value is not
-#pragma unroll
-    for (int h = 0; h < HD / 8; ++h)
-#pragma unroll
-      for (int j = 2 * i; j < 2 * i + 2; ++j) {
-        finite = fmaf(o[h][j], 0.0f, finite);
-        o[h][j] = l[i] == 0.0f ? 0.0f : o[h][j] * inv;
-      }
-    if (row_ok[i] && a.splits > 1) {
+    if (a.splits > 1) {
+      const long long at = static_cast<long long>(split) * a.B * a.Hq * a.Lq + head_row;
       if (t == 0) a.part_lse[at] = lse2;
       float2* po = reinterpret_cast<float2*>(a.part_o + at * HD) + t;
 #pragma unroll
-      for (int h = 0; h < HD / 8; ++h) po[4 * h] = make_float2(o[h][2 * i], o[h][2 * i + 1]);
-    } else if (row_ok[i]) {
+      for (int h = 0; h < HD / 8; ++h) po[4 * h] = make_float2(o[h][2 * i] * inv, o[h][2 * i + 1] * inv);
+    } else {
       if (t == 0 && a.lse != nullptr) a.lse[head_row] = lse2 * kLn2;
+      T* out = static_cast<T*>(a.out) + ((static_cast<long long>(b) * a.Lq + qi[i]) * a.Hq + qh[i]) * HD + 2 * t;
 #pragma unroll
       for (int h = 0; h < HD / 8; ++h)
-        *reinterpret_cast<uint32_t*>(out + 8 * h + 2 * t) = pack2(o[h][2 * i], o[h][2 * i + 1], T());
-    }
-    const bool again = row_ok[i] && !(finite == 0.0f) && l[i] > 0.0f && l[i] < INFINITY;
-    unsigned left = __ballot_sync(0xffffffffu, again);
-    while (left != 0) {
-      const int src = (__ffs(left) - 1) & ~3;  // the row's four lanes hold the same qi, qh and lse2
-      left &= ~(0xfu << src);
-      const int ri = __shfl_sync(0xffffffffu, qi[i], src), rh = __shfl_sync(0xffffffffu, qh[i], src);
-      const float rl = __shfl_sync(0xffffffffu, lse2, src);
-      const long long r = (static_cast<long long>(b) * a.Hq + rh) * a.Lq + ri;
-      __syncwarp();
-      if (a.splits > 1)
-        row_by_definition<T, HD, HD, BN>(a, sp, b, ri, rh, first, last, rl, 0,
-                                         a.part_o + (static_cast<long long>(split) * a.B * a.Hq * a.Lq + r) * HD);
-      else
-        row_by_definition<T, HD, HD, BN>(a, sp, b, ri, rh, first, last, rl, 0,
-                                         static_cast<T*>(a.out) + ((static_cast<long long>(b) * a.Lq + ri) * a.Hq + rh) * HD);
+        *reinterpret_cast<uint32_t*>(out + 8 * h) = pack2(o[h][2 * i] * inv, o[h][2 * i + 1] * inv, T());
     }
   }
 }
@@ -373,7 +364,7 @@ __global__ void __launch_bounds__(128) window_attn_kernel(const __grid_constant_
 constexpr int kAttnDecodeRows = 16, kAttnDecodeStages = 3;
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(128) window_attn_decode_kernel(const __grid_constant__ WindowAttnArgs a) {
+__global__ void __launch_bounds__(128) window_attn_decode_kernel(const WindowAttnArgs a) {
   using namespace attn;
   constexpr int BN = kAttnBN, WN = 16, KT = HD / 16, CH = HD / 8, D = kAttnDecodeStages;
   constexpr int TILE = WN * HD;  // values of a warp's K (or V) tile
@@ -438,16 +429,24 @@ __global__ void __launch_bounds__(128) window_attn_decode_kernel(const __grid_co
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
   const float sc = a.scale * kLog2e;
 
+  auto sees_all = [&](int j0) { return j0 + WN - 1 <= sp.p0 && (j0 > sp.p1 - a.window || j0 + WN <= a.sinks); };
+  bool cleared = false;  // of V, somewhere
   int stage = 0;
   for (int n = first; n < last; ++n) {
+    const int j0 = tile_key(n);
+    const bool whole = sees_all(j0);
     cp_wait<D - 2>();
+    if (!whole && sp.p0 != sp.p1) {  // (rows of one position see the same keys)
+#pragma unroll
+      for (int i = 0; i < WN * CH / 32; ++i)  // the chunks that this lane copied
+        cleared |= clear_not_finite<T>(ring + stage * (2 * TILE) + TILE + swz<HD>(lane / CH + i * (32 / CH), lane % CH));
+    }
     __syncwarp();  // the warp's copies have landed, and it is done with the stage that is filled next
     if (n + D - 1 < last) load(n + D - 1, stage == 0 ? D - 1 : stage - 1);
     cp_commit();
     const T* ks = ring + stage * (2 * TILE);
     const T* vs = ks + TILE;
     stage = stage == D - 1 ? 0 : stage + 1;
-    const int j0 = tile_key(n);
     if (j0 > sp.p1) continue;  // this warp's share of the last tile is behind every row
     float s[2][4] = {};
 #pragma unroll
@@ -457,7 +456,6 @@ __global__ void __launch_bounds__(128) window_attn_decode_kernel(const __grid_co
       mma(s[0], qf[kt], f[0], f[1], T());
       mma(s[1], qf[kt], f[2], f[3], T());
     }
-    const bool whole = j0 + WN - 1 <= sp.p0 && (j0 > sp.p1 - a.window || j0 + WN <= a.sinks);
     if (!whole) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -509,14 +507,16 @@ __global__ void __launch_bounds__(128) window_attn_decode_kernel(const __grid_co
     }
   }
 
+  if (__any_sync(0xffffffffu, cleared))
+    for (int n = first; n < last; ++n)
+      if (!sees_all(tile_key(n))) add_not_finite<T, HD, WN>(o, vb + 2 * t, a.v_t, tile_key(n), pos, a.window, a.sinks);
+
   // the four warps' results: [warp][row][HD] outputs, then maxima and sums
   constexpr int OP = HD + 8;  // row pitch: the rows of a store land in different banks
   float* po = reinterpret_cast<float*>(smem_raw);
   float* pm = po + 4 * kAttnDecodeRows * OP;
   float* pl = pm + 4 * kAttnDecodeRows;
-  float* redo = pl + 4 * kAttnDecodeRows;  // a row's log-sum-exp where it is computed again, else NaN
   __syncthreads();
-  if (threadIdx.x < kAttnDecodeRows) redo[threadIdx.x] = __int_as_float(0x7fc00000);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
@@ -532,7 +532,6 @@ __global__ void __launch_bounds__(128) window_attn_decode_kernel(const __grid_co
   }
   __syncthreads();
   constexpr int LANES = HD / 4;  // threads of a row, four values each
-  bool again = false;
   for (int r = threadIdx.x / LANES; r <= r1 - r0; r += 128 / LANES) {
     const int c = threadIdx.x % LANES * 4;
     float top = -INFINITY;
@@ -552,40 +551,17 @@ __global__ void __launch_bounds__(128) window_attn_decode_kernel(const __grid_co
     }
     const float inv = total > 0.0f ? 1.0f / total : (total == 0.0f ? 0.0f : total);
     const float lse2 = total == 0.0f ? -INFINITY : base + log2f(total);
-    float finite = 0.0f;  // NaN once a value is not
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      finite = fmaf(acc[i], 0.0f, finite);
-      acc[i] = total == 0.0f ? 0.0f : acc[i] * inv;
-    }
-    if (!(finite == 0.0f) && total > 0.0f && total < INFINITY) {
-      redo[r] = lse2;  // every thread of the row that finds one writes the same
-      again = true;
-    }
     const int qi = (r0 + r) / a.G, qh = hk * a.G + (r0 + r) % a.G;
     const long long head_row = (static_cast<long long>(b) * a.Hq + qh) * a.Lq + qi;
     if (a.splits > 1) {
       const long long at = static_cast<long long>(split) * a.B * a.Hq * a.Lq + head_row;
       if (c == 0) a.part_lse[at] = lse2;
       if (lse2 != -INFINITY)
-        *reinterpret_cast<float4*>(a.part_o + at * HD + c) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        *reinterpret_cast<float4*>(a.part_o + at * HD + c) = make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
     } else {
       if (c == 0 && a.lse != nullptr) a.lse[head_row] = lse2 * kLn2;
       T* out = static_cast<T*>(a.out) + ((static_cast<long long>(b) * a.Lq + qi) * a.Hq + qh) * HD + c;
-      *reinterpret_cast<uint2*>(out) = make_uint2(pack2(acc[0], acc[1], T()), pack2(acc[2], acc[3], T()));
-    }
-  }
-  if (__syncthreads_or(again)) {
-    for (int r = warp; r <= r1 - r0; r += 4) {
-      if (isnan(redo[r])) continue;
-      const int qi = (r0 + r) / a.G, qh = hk * a.G + (r0 + r) % a.G;
-      const long long head_row = (static_cast<long long>(b) * a.Hq + qh) * a.Lq + qi;
-      if (a.splits > 1)
-        row_by_definition<T, HD, HD, BN>(a, sp, b, qi, qh, first, last, redo[r], 0,
-                                         a.part_o + (static_cast<long long>(split) * a.B * a.Hq * a.Lq + head_row) * HD);
-      else
-        row_by_definition<T, HD, HD, BN>(a, sp, b, qi, qh, first, last, redo[r], 0,
-                                         static_cast<T*>(a.out) + ((static_cast<long long>(b) * a.Lq + qi) * a.Hq + qh) * HD);
+      *reinterpret_cast<uint2*>(out) = make_uint2(pack2(acc[0] * inv, acc[1] * inv, T()), pack2(acc[2] * inv, acc[3] * inv, T()));
     }
   }
 }
@@ -660,7 +636,7 @@ template <typename T, int HD>
 inline cudaError_t launch_window_attn(const WindowAttnArgs& a, cudaStream_t stream) {
   const long long rows = static_cast<long long>(a.Lq) * a.G;
   const bool decode = window_attn_decodes(rows);
-  constexpr int ring = 4 * kAttnDecodeStages * 2 * 16 * HD * 2, meet = 4 * kAttnDecodeRows * (HD + 8 + 2) * 4 + 4 * kAttnDecodeRows;
+  constexpr int ring = 4 * kAttnDecodeStages * 2 * 16 * HD * 2, meet = 4 * kAttnDecodeRows * (HD + 8 + 2) * 4;
   const int smem = decode ? (ring > meet ? ring : meet) : 4 * kAttnBN * HD * 2;
   const int per_tile = decode ? kAttnDecodeRows : kAttnRows;
   const auto kernel = decode ? window_attn_decode_kernel<T, HD> : window_attn_kernel<T, HD>;

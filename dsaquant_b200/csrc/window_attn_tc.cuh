@@ -23,8 +23,8 @@
 // it, and O is hardly ever rescaled.
 //
 // V rows of keys that no row of the CTA sees are overwritten with zeros in shared memory (by each tile's threads,
-// before they hand over P): 0 * garbage must not reach O.  What a key that only some rows see holds is dealt with at the
-// end (row_by_definition).  Every wait is bounded.
+// before they hand over P), and so are values that are not finite of keys that only some rows of the CTA see (the rows that see
+// them get them at the very end): 0 * inf must not reach O.  Every wait is bounded.
 //
 // Measured, 12 heads of 128 x 32760 queries, window 4096, 64 first keys, bf16: 850 us, 0.786 TFLOP at 925 TFLOP/s, 0.56 of the
 // library product's burst rate (the mma.sync form: 2842 us).  Tensor pipe and special-function unit are each 46 % busy:
@@ -133,7 +133,7 @@ __device__ __forceinline__ bool tile_active(int p0, int p1, int j0, int window, 
 template <typename T, int HD>
 __global__ void __launch_bounds__(AttnTcCfg<HD>::THREADS, 1)
 window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttnTcParams prm) {
+                      const __grid_constant__ CUtensorMap tm_v, const AttnTcParams prm) {
   using namespace attn;
   using C = AttnTcCfg<HD>;
   const WindowAttnArgs& a = prm.a;
@@ -151,6 +151,8 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
   auto bar_p = [&](int x, uint32_t buf) { return bar0 + 8u * (2 * C::S + 5 + 2 * x + buf); };
   auto bar_o = [&](int x, uint32_t buf) { return bar0 + 8u * (2 * C::S + 9 + 2 * x + buf); };
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + C::OFF_BAR + 8 * C::NUM_BARS);
+  // set before the first value is cleared; the CTA reads it behind its last barrier
+  volatile int* cleared = reinterpret_cast<volatile int*>(gen + C::OFF_BAR + 8 * C::NUM_BARS + 4);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(gen + C::OFF_BAR + 8 * C::NUM_BARS + 8);
   auto wait = [&](uint32_t bar, uint32_t parity) {
     return ptx::mbar_probe(bar, parity) || wait_longer(bar, parity, abort_flag, prm.status, prm.abort_word, prm.launch_id);
@@ -171,6 +173,7 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
       ptx::mbar_init(bar_o(x, 1), 1);
     }
     *abort_flag = 0;
+    *cleared = 0;
     ptx::fence_mbar_init();
   }
   if (warp == C::WARP_MMA) {
@@ -366,23 +369,6 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
 #pragma unroll
         for (int i = 0; i < 32; ++i)
           if (!(seen >> i & 1)) s[i] = 0xff800000u;
-        const bool cover = j0 + C::BN - 1 <= sp.hi && (j0 >= sp.lo || j0 + C::BN <= a.sinks);
-        if (!cover) {
-          const uint32_t at = n + 1 < sp.n ? 2 * n + 2 : 2 * n + 1, slot = at % C::S;  // V(n) in the ring
-          const bool here = wait(bar_full(slot), (at / C::S) & 1);
-          alive &= here;
-          const int row = r & 63, j = j0 + row;
-          if (here && !(j <= sp.hi && (j >= sp.lo || j < a.sinks))) {
-#pragma unroll
-            for (int c = 0; c < HD / 64; ++c)
-#pragma unroll
-              for (int i = 0; i < 2; ++i)
-                detail::sts128(base + C::OFF_RING + slot * C::K_TILE + c * C::K_ATOM + row * 128 +
-                                   16 * (i + 2 * (r >> 6) + 4 * h),
-                               make_uint4(0, 0, 0, 0));
-          }
-          ptx::fence_proxy_async_smem();
-        }
       }
       // Weights against the maximum known so far.  A row that has none yet, or whose weights of this tile add up to
       // over 2^9 in one half (the only sign that the maximum moved far), makes its warps find the maximum and do
@@ -456,6 +442,32 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         ptx::tmem_st_wait();  // the weights are written again
       }
       l += sum;
+#pragma unroll 1
+      for (bool edge = !whole; edge; edge = false) {  // behind the weights: V(n) has had their time to arrive
+        const uint32_t at = n + 1 < sp.n ? 2 * n + 2 : 2 * n + 1, slot = at % C::S;  // V(n) in the ring
+        const bool here = wait(bar_full(slot), (at / C::S) & 1);
+        alive &= here;
+        bool wrote = false;
+        if (here) {
+          const int row = r & 63, j = j0 + row;
+          const bool covered = j <= sp.hi && (j >= sp.lo || j < a.sinks);  // by some row
+#pragma unroll
+          for (int c = 0; c < HD / 64; ++c)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              uint8_t* chunk = gen + C::OFF_RING + slot * C::K_TILE + c * C::K_ATOM + row * 128 + 16 * (i + 2 * (r >> 6) + 4 * h);
+              if (!covered) {
+                *reinterpret_cast<uint4*>(chunk) = make_uint4(0, 0, 0, 0);
+                wrote = true;
+              } else if (any_not_finite<T>(chunk)) {
+                *cleared = 1;
+                __threadfence_block();
+                wrote |= clear_not_finite<T>(chunk);
+              }
+            }
+        }
+        if (wrote) ptx::fence_proxy_async_smem();
+      }
       ptx::tmem_st_wait();
       ptx::tc_fence_before_sync();
       __syncwarp();
@@ -469,14 +481,10 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     }
     l = exchange(l, [](float u, float v) { return u + v; });
     const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-    const float lse2 = l == 0.0f ? -INFINITY : m + log2f(l);
     const bool ok = qi < a.Lq && alive;
-    if (h == 0 && ok && a.lse != nullptr) a.lse[(static_cast<long long>(b) * a.Hq + hq) * a.Lq + qi] = lse2 * kLn2;
-    auto out_of = [&](int query) {
-      return static_cast<T*>(a.out) + ((static_cast<long long>(b) * a.Lq + query) * a.Hq + hq) * HD + h * (HD / 2);
-    };
-    T* out = out_of(qi);
-    float finite = 0.0f;  // NaN once a value is not
+    if (h == 0 && ok && a.lse != nullptr)
+      a.lse[(static_cast<long long>(b) * a.Hq + hq) * a.Lq + qi] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+    T* out = static_cast<T*>(a.out) + ((static_cast<long long>(b) * a.Lq + qi) * a.Hq + hq) * HD + h * (HD / 2);
 #pragma unroll 1
     for (int c = 0; c < HD / 64; ++c) {
       uint32_t o[32];
@@ -484,12 +492,6 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         ptx::tmem_ld_32x32(t_o + 32 * c, o);
         ptx::tmem_ld_wait_for(o);
       } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = 0u;
-      }
-#pragma unroll
-      for (int i = 0; i < 32; ++i) finite = fmaf(__uint_as_float(o[i]), 0.0f, finite);
-      if (l == 0.0f) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) o[i] = 0u;
       }
@@ -504,14 +506,6 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         }
       }
     }
-    unsigned left = __ballot_sync(0xffffffffu, ok && !(finite == 0.0f) && l > 0.0f && l < INFINITY);
-    __syncwarp();
-    for (; left != 0; left &= left - 1) {
-      const int src = __ffs(left) - 1;
-      const int query = i0 + x * C::BM + (warp & 3) * 32 + src;
-      row_by_definition<T, HD, HD / 2, C::BN>(a, sp, b, query, hq, 0, sp.n, __shfl_sync(0xffffffffu, lse2, src), h * (HD / 2),
-                                              out_of(query));
-    }
   }
 
   ptx::tc_fence_before_sync();
@@ -520,6 +514,34 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     __syncwarp();
     ptx::tc_fence_after_sync();
     ptx::tmem_dealloc<1>(tmem, C::TMEM_COLS);
+  }
+  if (*cleared != 0 && *abort_flag == 0 && warp < C::SOFTMAX_WARPS) {
+    // each warp its rows and columns, a lane a column (or two) of one row after another
+    const int x = warp >> 3, h = (warp >> 2) & 1;
+    const T* v = static_cast<const T*>(a.v) + b * a.v_b + (hq / a.G) * a.v_h + h * (HD / 2) + lane;
+#pragma unroll 1
+    for (int r = 0; r < 32; ++r) {
+      const int qi = i0 + x * C::BM + (warp & 3) * 32 + r, p = sp.p0 + qi - i0;
+      if (qi > i1) break;
+      float bad[HD / 64] = {};
+      for (int n = 0; n < sp.n; ++n) {
+        const int j0 = tile_key(n);
+        if (j0 + C::BN - 1 <= sp.p0 && (j0 > sp.p1 - a.window || j0 + C::BN <= a.sinks)) continue;  // all rows see all of it
+#pragma unroll 4
+        for (int j = j0; j < j0 + C::BN; ++j) {
+          if (!(j <= p && (j > p - a.window || j < a.sinks))) continue;
+#pragma unroll
+          for (int c = 0; c < HD / 64; ++c) {
+            const float y = static_cast<float>(v[j * a.v_t + 32 * c]);
+            if (!(fabsf(y) < INFINITY)) bad[c] += y;
+          }
+        }
+      }
+      T* out = static_cast<T*>(a.out) + ((static_cast<long long>(b) * a.Lq + qi) * a.Hq + hq) * HD + h * (HD / 2) + lane;
+#pragma unroll
+      for (int c = 0; c < HD / 64; ++c)
+        if (bad[c] != 0.0f) out[32 * c] = static_cast<T>(static_cast<float>(out[32 * c]) + bad[c]);
+    }
   }
 }
 
