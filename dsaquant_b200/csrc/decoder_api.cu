@@ -91,7 +91,7 @@ int b200w4a4_rms_norm_quant(const void* x, int x_dtype, long long x_ld, const vo
 int b200w4a4_quantize_weight_grouped(const void* w, int w_dtype, void* packed, void* scale, int N,
                                      int K, int group, void* stream) {
   if (w == nullptr || packed == nullptr || scale == nullptr || !float_dtype(w_dtype)) return B200W4A4_EINVAL;
-  if (N < 1 || K < 32 || group < 32 || group % 32 != 0 || K % group != 0) return B200W4A4_ESHAPE;
+  if (N < 1 || K < 32 || group < 32 || group % 32 != 0 || K % group != 0 || K > (1 << 20)) return B200W4A4_ESHAPE;
   if (!aligned(w, size_of(w_dtype)) || !aligned(scale, 2)) return B200W4A4_EALIGN;
   const int rc = current_device(nullptr);
   if (rc != B200W4A4_OK) return rc;
@@ -113,7 +113,7 @@ int b200w4a4_linear_w4_group(const void* x, int x_dtype, const float* act_scale,
   out_dtype &= ~B200W4A4_BIAS_F32;
   if (out_dtype != B200W4A4_F16 && out_dtype != B200W4A4_BF16) return B200W4A4_EINVAL;
   if (M < 0 || N < 1 || K < 32 || group < 32 || group % 32 != 0 || K % group != 0) return B200W4A4_ESHAPE;
-  if (M > 65535 * 8 || K > (1 << 20)) return B200W4A4_ESHAPE;
+  if (M > 65535 * 8 || K > (1 << 20) || N > 0x7fffffff - 511) return B200W4A4_ESHAPE;  // row numbers of the last block are 32 bits
   if (M == 0) return B200W4A4_OK;
   if (x == nullptr || packed == nullptr || scale == nullptr || out == nullptr) return B200W4A4_EINVAL;
   if ((x_dtype == B200W4A4_X_INT8) != (act_scale != nullptr)) return B200W4A4_EINVAL;

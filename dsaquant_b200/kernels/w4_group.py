@@ -20,6 +20,7 @@ from .vdm_w4a4 import _DTYPE_CODE, _empty, _load_ext, _require_cuda, _run, _stre
 
 _X_CODE = {torch.float16: 0, torch.bfloat16: 1, torch.int8: 3}
 MAX_TOKENS = 65535 * 8
+MAX_ROWS, MAX_WIDTH = (1 << 31) - 512, 1 << 20  # of the weight (the foreign calls take 32-bit sizes)
 _OUT_CODE = {torch.float16: 0, torch.bfloat16: 1}
 _BIAS_F32 = 16
 
@@ -35,6 +36,8 @@ def quantize_weight_grouped(weight: torch.Tensor, group_size: int = 128) -> Tupl
     n, k = weight.shape
     if n < 1 or group_size < 32 or group_size % 32 or k < 1 or k % group_size:
         raise ValueError("group_size must be a multiple of 32 that divides K")
+    if n > MAX_ROWS or k > MAX_WIDTH:
+        raise ValueError(f"a weight has at most {MAX_ROWS} rows of {MAX_WIDTH} values")
     w = weight.detach().contiguous()
     packed = torch.empty((n, k // 2), dtype=torch.uint8, device=w.device)
     scales = torch.empty((n, k // group_size), dtype=torch.float16, device=w.device)
@@ -87,6 +90,8 @@ def linear_w4_group(
         raise ValueError(f"the last dimension of x must be K={k}")
     if n < 1 or k < 1 or scales.shape[0] != n or groups < 1 or k % groups or (k // groups) % 32:
         raise ValueError("scales must be [N, K/group] with a group that is a multiple of 32 and divides K")
+    if n > MAX_ROWS or k > MAX_WIDTH:
+        raise ValueError(f"a weight has at most {MAX_ROWS} rows of {MAX_WIDTH} values")
     dev = x.device
     if packed.device != dev or scales.device != dev:
         raise ValueError("x, packed and scales must be on one device")

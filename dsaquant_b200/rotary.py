@@ -13,6 +13,7 @@ import torch
 from . import _lib
 from .kernels.vdm_w4a4 import _DTYPE_CODE, _empty, _load_ext, _require_cuda, _run, _stream_ptr
 
+MAX_HEADS = 65536
 SCALINGS = ("none", "linear", "ntk", "yarn")
 
 
@@ -145,8 +146,8 @@ def apply_rotary(
         raise ValueError("positions must be int32 or int64 with one value for each token")
     if cos_sin.device != dev or positions.device != dev:
         raise ValueError("q, cos_sin and positions must be on one device")
-    if hq < 1 or (k is not None and hk < 1):
-        raise ValueError("q and k must have heads")
+    if not 1 <= hq <= MAX_HEADS or (k is not None and not 1 <= hk <= MAX_HEADS):
+        raise ValueError(f"q and k must have 1 to {MAX_HEADS} heads")
     if inplace and t > 0 and not (_distinct(q) and (k is None or (_distinct(k) and _disjoint(q, k)))):
         raise ValueError("inplace needs q and k whose tokens and heads share no memory, with one another either")
     q_out, k_out = (q, k) if inplace else (_empty((t, hq, hd), dtype, dev), None)

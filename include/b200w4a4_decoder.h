@@ -47,7 +47,7 @@ int b200w4a4_quantize_weight_grouped(const void* w, int w_dtype, void* packed, v
  * (act_scale NULL), or int8 when x_dtype is B200W4A4_X_INT8 (act_scale fp32 [M]).  packed and
  * scale as b200w4a4_quantize_weight_grouped writes them.  out [M, N] and bias [N] (or NULL) are of
  * out_dtype (F16 or BF16); with out_dtype | B200W4A4_BIAS_F32 the bias is fp32 and added as it is.  Products are exact, sums are fp32 (int32 within a group for int8).
- * M <= 524280, K <= 1048576. */
+ * M <= 524280, N <= 2^31 - 512, K <= 1048576. */
 #define B200W4A4_X_INT8 3
 #define B200W4A4_BIAS_F32 16
 int b200w4a4_linear_w4_group(const void* x, int x_dtype, const float* act_scale, const void* packed,

@@ -272,3 +272,10 @@ def test_yarn_ramp_is_linear_in_the_pair():
         f, ramp = base ** (-2 * i / rd), min(max((i - low) / (high - low), 0.0), 1.0)
         want = f * (1 - ramp) + f / factor * ramp
         assert abs(math.atan2(table[1, i, 1], table[1, i, 0]) - want) < 2.0 ** -22
+
+
+@pytest.mark.parametrize("over, code", [(dict(n=(1 << 31) - 1), -2), (dict(n=(1 << 31) - 511), -2), (dict(k=(1 << 20) + 128), -2)])
+def test_linear_w4_group_refuses_sizes_past_its_row_numbers(lib, over, code):
+    """A last block of rows past 2^31 would wrap."""
+    assert _w4(lib, **over) == code
+    assert lib.b200w4a4_quantize_weight_grouped(P, 0, P, P, 4, (1 << 20) + 32, 32, None) == -2

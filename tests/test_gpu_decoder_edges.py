@@ -404,3 +404,27 @@ def test_linear_w4_group_adds_the_bias_as_it_is(xdtype, out_dtype, bias_dtype):
         x, act = (x * 100).round().clamp(-128, 127).to(torch.int8), torch.full((5,), 0.001, device="cuda")
     _check_w4(x, packed, scales, bias, act, out_dtype)
     _check_w4(x, packed, scales, bias.repeat_interleave(2)[::2], act, out_dtype)
+
+
+def test_sizes_that_32_bits_do_not_hold_are_refused():
+    """The foreign calls take 32-bit sizes and cut larger ones off."""
+    from dsaquant_b200.kernels.w4_group import linear_w4_group, quantize_weight_grouped
+    from dsaquant_b200.rotary import apply_rotary, rotary_table
+
+    def big(dtype, *shape):
+        return torch.zeros(1, device="cuda", dtype=dtype).expand(shape)
+
+    k = (1 << 32) + 64
+    with pytest.raises(ValueError, match="at most"):
+        linear_w4_group(big(BF, 1, k), big(torch.uint8, 1, k // 2), big(FP, 1, k // 64))
+    with pytest.raises(ValueError, match="at most"):
+        linear_w4_group(big(BF, 1, 64), big(torch.uint8, (1 << 32) + 5, 32), big(FP, (1 << 32) + 5, 1))
+    for n, width in ((1, k), ((1 << 32) + 5, 64)):
+        with pytest.raises(ValueError, match="at most"):
+            quantize_weight_grouped(big(BF, n, width), 64)
+    table, pos = rotary_table(4, 2, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    few = torch.zeros(1, 2, 2, device="cuda", dtype=BF)
+    many = few[:, :1].expand(1, (1 << 32) + 1, 2)
+    for q, kk in ((many, None), (few, many)):
+        with pytest.raises(ValueError, match="heads"):
+            apply_rotary(q, kk, table, pos)
