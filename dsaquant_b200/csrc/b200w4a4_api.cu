@@ -890,7 +890,9 @@ int b200w4a4_last_device_status(int device) {
   if (rc == B200W4A4_OK) {
     if (cudaDeviceSynchronize() != cudaSuccess ||
         cudaMemcpy(&value, st->status_ptr, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess ||
-        cudaMemset(st->status_ptr, 0, sizeof(int)) != cudaSuccess)
+        cudaMemset(st->status_ptr, 0, sizeof(int)) != cudaSuccess ||
+        // nothing runs now; a captured launch keeps its id, and its replays must not go on giving up unreported
+        cudaMemset(st->abort_ptr, 0, sizeof(unsigned)) != cudaSuccess)
       rc = B200W4A4_ECUDA;
   }
   cudaSetDevice(prev);
