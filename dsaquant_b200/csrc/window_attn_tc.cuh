@@ -23,8 +23,10 @@
 // it, and O is hardly ever rescaled.
 //
 // V rows of keys that no row of the CTA sees are overwritten with zeros in shared memory (by each tile's threads,
-// before they hand over P), and so are values that are not finite of keys that only some rows of the CTA see (the rows that see
-// them get them at the very end): 0 * inf must not reach O.  Every wait is bounded.
+// before they hand over P), and so are values that are not finite in the key tiles that some row of the CTA does not see
+// entirely (the rows that see them get them at the very end): 0 * inf must not reach O.  Both tiles do so in the same key tiles,
+// also where all rows of one of them see every key: its product would else meet such a value or a zero, by which tile came
+// first.  Every wait is bounded.
 //
 // Measured, 12 heads of 128 x 32760 queries, window 4096, 64 first keys, bf16: 850 us, 0.786 TFLOP at 925 TFLOP/s, 0.56 of the
 // library product's burst rate (the mma.sync form: 2842 us).  Tensor pipe and special-function unit are each 46 % busy:
@@ -209,6 +211,8 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     while (n <= last && !tile_active(first_pos(x), last_pos(x), tile_key(n), a.window, a.sinks)) ++n;
     return n;
   };
+  // whether every row of the CTA sees all keys of the tile from j0 on
+  auto cta_sees = [&](int j0) { return j0 + C::BN - 1 <= sp.p0 && (j0 > sp.p1 - a.window || j0 + C::BN <= a.sinks); };
   const int to_a = last_tile(0), to_b = last_tile(1), from_a = first_tile(0, to_a), from_b = first_tile(1, to_b);
   auto active = [&](int x, int n) {
     const int to = x == 0 ? to_a : to_b, from = x == 0 ? from_a : from_b;
@@ -443,11 +447,10 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
       }
       l += sum;
 #pragma unroll 1
-      for (bool edge = !whole; edge; edge = false) {  // behind the weights: V(n) has had their time to arrive
+      for (bool edge = !cta_sees(j0); edge; edge = false) {  // behind the weights: V(n) has had their time to arrive
         const uint32_t at = n + 1 < sp.n ? 2 * n + 2 : 2 * n + 1, slot = at % C::S;  // V(n) in the ring
         const bool here = wait(bar_full(slot), (at / C::S) & 1);
         alive &= here;
-        bool wrote = false;
         if (here) {
           const int row = r & 63, j = j0 + row;
           const bool covered = j <= sp.hi && (j >= sp.lo || j < a.sinks);  // by some row
@@ -458,15 +461,15 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
               uint8_t* chunk = gen + C::OFF_RING + slot * C::K_TILE + c * C::K_ATOM + row * 128 + 16 * (i + 2 * (r >> 6) + 4 * h);
               if (!covered) {
                 *reinterpret_cast<uint4*>(chunk) = make_uint4(0, 0, 0, 0);
-                wrote = true;
               } else if (any_not_finite<T>(chunk)) {
                 *cleared = 1;
                 __threadfence_block();
-                wrote |= clear_not_finite<T>(chunk);
+                clear_not_finite<T>(chunk);
               }
             }
         }
-        if (wrote) ptx::fence_proxy_async_smem();
+        // Whoever wrote: what the other tile cleared may have been read here as finite already.
+        ptx::fence_proxy_async_smem();
       }
       ptx::tmem_st_wait();
       ptx::tc_fence_before_sync();
@@ -526,7 +529,7 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
       float bad[HD / 64] = {};
       for (int n = 0; n < sp.n; ++n) {
         const int j0 = tile_key(n);
-        if (j0 + C::BN - 1 <= sp.p0 && (j0 > sp.p1 - a.window || j0 + C::BN <= a.sinks)) continue;  // all rows see all of it
+        if (cta_sees(j0)) continue;
 #pragma unroll 4
         for (int j = j0; j < j0 + C::BN; ++j) {
           if (!(j <= p && (j > p - a.window || j < a.sinks))) continue;

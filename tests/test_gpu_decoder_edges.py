@@ -212,6 +212,28 @@ def test_window_attention_not_finite_values_reach_only_the_rows_that_see_them(lq
     assert torch.equal(clean, window_attention(q, k, v, window, sinks, kv_lens=kv_lens))
 
 
+@pytest.mark.parametrize("dtype, hd", [(FP, 64), (BF, 128)])
+def test_window_attention_infinite_value_of_no_weight_in_the_blocks_edge(dtype, hd):
+    """256 queries share a block, two tiles of 128.  Keys that every row of one tile sees and only some of the other are the block's
+    edge for both: an infinite value there is added to the rows that see it, never multiplied with a weight that came out as 0,
+    whichever tile gets to it first."""
+    from dsaquant_b200.window_attention import window_attention
+
+    g = _gen(64)
+    b, lq, lk, heads, window = 4, 256, 1000, 24, 300
+    q, k, v = _qkv(g, b, lq, lk, heads, heads, hd, dtype)
+    at = lk - lq + torch.arange(lq, device="cuda")
+    for key in (580, 639, 640, 703, 704, 767, 768, 831):              # 576 .. 703 the first tile sees whole, 704 .. 831 the second
+        bad_q, bad_k, bad = q.clone(), k.clone(), v.clone()
+        bad_q[..., 0], bad_k[:, key, :, 0], bad[:, key, :, 5] = 16.0, -200.0, float("inf")    # a score of -280 and less: a weight of 0 in fp32
+        sees = (at >= key) & (at < key + window)
+        first = window_attention(bad_q, bad_k, bad, window)
+        assert bool((first[:, sees, :, 5] == float("inf")).all())
+        assert bool(torch.isfinite(first[:, ~sees]).all()) and bool(torch.isfinite(first[..., :5]).all()) and bool(torch.isfinite(first[..., 6:]).all())
+        for _ in range(5):
+            assert torch.equal(first.view(torch.int16), window_attention(bad_q, bad_k, bad, window).view(torch.int16))
+
+
 def test_window_attention_every_value_not_finite():
     """A whole prompt of NaN is slow at worst: it ends, rows that see nothing are 0, all others NaN."""
     from dsaquant_b200.kernels import vdm_w4a4 as vdm
