@@ -6,9 +6,11 @@
 // The row is loaded once and stays in registers as fp32 through both reductions (sum of squares,
 // abs-max), so what moves is x, the residual in and out, one byte a value and four a row.
 //
-// Measured at 32760 x 5120 bf16 with residual: int8 179 us (6.55 TB/s on 7 bytes a value, 1.01 of the copy rate), e4m3 232 us;
-// fp16 without residual 112 us (4.5 TB/s: bound by the instructions between load and store).  Rows whose length or address
-// allows no 128-bit access move one value an access: 20000 x 5121 with residual 445 us, four times the copy.
+// Measured at 32760 x 5120 bf16 with residual: int8 180 us (6.51 TB/s on 7 bytes a value, 1.01 of the copy rate), e4m3 203 us;
+// fp16 without residual int8 119 us (4.2 TB/s: the schedulers issue in 76 % of their cycles, the code conversions among it; codes by
+// a reciprocal alone, off by one beside a border, took 110), e4m3 143 us.  Rows whose length or address allows no
+// 128-bit access move one value an access: 20000 x 5121 with residual 439 us, four times the copy.  Worst case: a
+// row of equal values in e4m3 is all largest values (32760 x 5120: 381 us).
 //
 // e4m3 codes are those of the exact quotient: its midpoints are 2^-4 of a value apart, so among millions of values
 // some always lie within the fp32 roundings of one, and a code on the wrong side is a step of 6 %.  So every value is
@@ -183,7 +185,7 @@ __global__ void __launch_bounds__(256, NCH <= 5 ? 4 : 2) rms_norm_quant_kernel(c
     if (rr != nullptr && row_ok) {
 #pragma unroll
       for (int i = 0; i < NCH; ++i) {
-        float r[8];  // the residual may be overwritten: a chunk's loads come before its stores
+        float r[8];  // a chunk's loads come before its stores
 #pragma unroll
         for (int e = 0; e < 8; ++e) r[e] = at(i, e) < a.D ? detail::load_f32(rr + at(i, e)) : 0.0f;
 #pragma unroll
@@ -346,7 +348,7 @@ inline cudaError_t launch_rms_norm_quant_as(const RmsNormArgs& a, cudaStream_t s
   } while (0)
   const int chunks = (a.D + 7) / 8;
   // Threads a row by its length; four blocks of 256 threads an SM while 40 values a thread allow it (32760 x 5120 fp16
-  // without residual: 112 us, 139 with 24 values and 256 threads a row).
+  // without residual: 119 us, 155 with 24 values and 256 threads a row).
   if (chunks <= 32) B200W4A4_RMS_LAUNCH(32, 1);
   else if (chunks <= 32 * 3) B200W4A4_RMS_LAUNCH(32, 3);
   else if (chunks <= 64 * 3) B200W4A4_RMS_LAUNCH(64, 3);

@@ -18,10 +18,10 @@
 // total with the group's scale.  The warps of a CTA share its rows and split K; their totals are
 // added in shared memory in a fixed order.
 //
-// Measured (device time, weights past L2): 1 x 5120 -> 15360 bf16, groups of 128: 16.7 us (2.4 TB/s of weight and scales;
-// the copy rate would take 6.3); 8 x 13824 -> 5120 fp16, groups of 64: 18.2 us; 5 x 1536 -> 8960 int8, groups of 32: 7.0 us.  The
-// ALU is 62 % busy with the masks while the SMs are, half of the stalls wait for memory, and a call this short spends
-// some 3 us on its launch and last wave.  Slower, each measured at the first shape against the form of its time:
+// Measured (device time, weights past L2): 1 x 5120 -> 15360 bf16, groups of 128: 18.1 us (2.2 TB/s of weight and scales;
+// the copy rate would take 6.3); 8 x 13824 -> 5120 fp16, groups of 64: 19.6 us; 5 x 1536 -> 8960 int8, groups of 32: 8.1 us.  The
+// ALU is 59 % busy with the masks while the SMs are, half of the stalls wait for memory, DRAM is 24 % busy, and a call this
+// short spends some 3 us on its launch and its last wave (2.16 waves of blocks at the first shape).  Slower, each measured at the first shape against the form of its time:
 // the same stream through a per-warp cp.async ring in shared memory (27 us) or a register ring (27), leaving the bias of the
 // pairs in and taking it out through a product with ones (24), shifts as multiplications' high words (21).
 #pragma once
@@ -111,7 +111,8 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[WORDS
 }  // namespace detail
 
 constexpr int kW4Warps = 8;
-// At most so many warps an SM when K is split: 1 x 5120 -> 15360 takes 18.9 us with 48 (K in four), 18.0 with 64 (in eight).
+// At most so many warps an SM are asked for when K is split; up to eight tokens 24 are resident, so this is 2.2 waves of blocks:
+// 1 x 5120 -> 15360 takes 18.9 us with 48 (K in four, 1.1 waves of longer blocks), 18.0 with 64 (in eight).
 constexpr int kW4WarpsPerSm = 64;
 
 // GB: codes that are sure to share a scale (32, 64 or 128; a divisor of the group).  A superblock is

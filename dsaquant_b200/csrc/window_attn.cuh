@@ -168,6 +168,9 @@ __device__ __forceinline__ void add_not_finite(float (&o)[HD / 8][4], const T* v
 
 // Short chunks (more rows than the single-token kernel takes, fewer than 128 queries), and prompts whose pitches no
 // tensor map can express: mma.sync, four warps of 16 rows each, key tiles of 64 in two cp.async stages.
+// Measured: 2 x 60 queries on 8000 keys, 8 heads of 128: 35 us; 8 x 127 on up to 8000 keys, 12 heads: 147; 32 x 127 on 16000
+// keys, 40 query and 8 key heads: 4.85 ms, 0.27 PFLOP/s.  What bounds it is mma.sync: every warp reads each key tile again
+// from shared memory, for 16 rows.
 constexpr int kAttnRows = 64, kAttnBN = 64;
 
 template <typename T, int HD>
@@ -359,8 +362,9 @@ __global__ void __launch_bounds__(128) window_attn_kernel(const WindowAttnArgs a
 // Single tokens: at most 16 rows a tile.  What bounds it is reading the keys and values once, so a CTA's four warps
 // each take 16 keys of every 64-key tile through a ring of their own (cp.async, kAttnDecodeStages deep, no barrier
 // between the warps), keep their own maximum, sum and output, and meet at the end in shared memory.
-// Measured, 16 sequences of 0 to 8192 keys, 40 query and 8 key heads of 128, window 4096: 42 us with the joining kernel
-// for 206 MB (4.9 TB/s, 0.76 of the copy rate); the 64-row form above took 67.5.
+// Measured, 16 sequences of 0 to 8192 keys, 40 query and 8 key heads of 128, window 4096: 44 us with the joining kernel
+// for 206 MB (4.7 TB/s, 0.72 of the copy rate); the 64-row form above took 67.5.  96 KB of ring allow two blocks an SM, whose
+// blocks of unequal length come in 2.2 waves.
 constexpr int kAttnDecodeRows = 16, kAttnDecodeStages = 3;
 
 template <typename T, int HD>

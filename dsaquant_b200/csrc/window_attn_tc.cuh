@@ -28,10 +28,11 @@
 // also where all rows of one of them see every key: its product would else meet such a value or a zero, by which tile came
 // first.  Every wait is bounded.
 //
-// Measured, 12 heads of 128 x 32760 queries, window 4096, 64 first keys, bf16: 850 us, 0.786 TFLOP at 925 TFLOP/s, 0.56 of the
-// library product's burst rate (the mma.sync form: 2842 us).  Tensor pipe and special-function unit are each 46 % busy:
-// what is left is latency between the roles, instruction fetch (four roles share the caches) and a tenth in a
-// block's start and end.
+// Measured, 12 heads of 128 x 32760 queries, window 4096, 64 first keys, bf16: 821 us in bursts of a few calls, 0.786 TFLOP at
+// 957 TFLOP/s, 0.58 of the library product's burst rate (the mma.sync form: 2842 us); call after call for seconds 933 us.
+// Tensor pipe and special-function unit are each 44 % busy: what is left is latency between the roles, instruction fetch
+// (four roles share the caches) and a tenth in a block's start and end.  Clearing values of V that are not finite is in it
+// (810 us without, when such a value made rows NaN that do not see it).
 #pragma once
 #include <cuda.h>
 
@@ -46,7 +47,10 @@
 namespace b200w4a4 {
 
 constexpr int DEV_TIMEOUT_ATTENTION = 106;
-// From one full tile of queries on.  Three chunks of 517 queries (8 heads of 64, window 300): 16.9 us, mma.sync form 19.2.
+// From one full tile of queries on.  Measured against the mma.sync form: 32 x 128 queries on 4096 keys, 40 query and 8 key heads
+// of 128: 494 and 1263 us; 8 x 128 of them: 166 and 376; 512 on 512: 21 and 38; 3 x 517, 8 heads of 64, window 300: 19.9 and 20.2.
+// The rule does not ask how many blocks there are, and this form never splits the keys: where a call is a few blocks the
+// other one would be faster (128 queries, 12 heads: 10.1 and 8.4 us on 128 keys, 55 and 28 on 4096; 8 heads on 32768 keys: 381 and 81).
 constexpr int kAttnTcMinQueries = 128;
 
 template <int HD>

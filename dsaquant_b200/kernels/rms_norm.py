@@ -39,7 +39,8 @@ def rms_norm_quant(
         scale = max(max|y|, 1e-5) / top * clip_ratio      top = 127 for torch.int8, 448 for torch.float8_e4m3fn
         codes = clamp(rint(y / scale), -128, 127)         or y / scale rounded to e4m3, saturating
 
-    Everything is fp32 and reads s before its rounding.  D is at most 16384.  Rows may be strided (views of a
+    Everything is fp32 and reads s before its rounding: int8 codes are those of the fp32 quotient by the scale that is returned,
+    e4m3 codes those of the exact quotient (values beside a border are decided in 64 bits).  D is at most 16384.  Rows may be strided (views of a
     wider tensor are read in place).  A row whose sum of squares is not finite in fp32 (it
     holds an infinity, a NaN, or values near 1e19), whose mean square and eps add up to less than fp32's normal range (values
     below 1e-19 with an eps of 0), or whose scale leaves 1.2e-38 .. 8.5e37 has scale NaN and codes 0.  Forward only, as every operator here."""

@@ -10,7 +10,8 @@ from . import _lib
 from .kernels.vdm_w4a4 import _empty, _load_ext, _require_cuda, _run, _stream_ptr
 
 _CODE = {torch.float16: 0, torch.bfloat16: 1}
-PROMPT_QUERIES = 128  # from here on a call takes the kernel for prompts, which needs no workspace
+# from here on a call takes the kernel for prompts, which needs no workspace (kAttnTcMinQueries; a test holds the two together)
+PROMPT_QUERIES = 128
 
 
 def _readable(x: torch.Tensor) -> Tuple[torch.Tensor, Tuple[int, ...]]:
@@ -47,8 +48,11 @@ def window_attention(
     kv_lens (int32 [B]; None: Lk) are the valid keys of each sequence, the queries its last Lq positions: query i is
     at p = kv_len - Lq + i and sees keys j <= p with j > p - window or j < sinks.  A window of Lk or more is plain
     causal attention.  A query that sees nothing (p < 0) gives 0, and -inf for the log-sum-exp.  Keys that no
-    query sees may hold anything.  scale: by default head_dim ** -0.5.  Strides are free where they are
-    multiples of 16 bytes with unit stride in the head; other tensors are copied first."""
+    query sees may hold anything, and a value that is not finite in a key that some queries see reaches those alone (a NaN
+    in k all of their output, one in v its own column).  scale: by default head_dim ** -0.5.  Scores, sums and outputs are
+    held in fp32; the softmax weights are rounded to q's type before they multiply v, which is most of the error beside the
+    output's own rounding.  Strides are free where they are multiples of 16 bytes with unit stride in the head; other
+    tensors are copied first."""
     lib = _load_ext()
     _require_cuda(q, "q")
     if q.dtype not in _CODE:

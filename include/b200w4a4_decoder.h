@@ -26,7 +26,8 @@ extern "C" {
  * x, residual [M, D] of x_dtype (F16, BF16, F32), row pitches x_ld / residual_ld; weight [D] of
  * w_dtype; codes [M, D] bytes; scale fp32 [M]; residual_out [M, D] of x_dtype = s rounded once.
  * residual and residual_out are both given or both NULL.  The arithmetic is fp32 and reads s before its
- * rounding; e4m3 codes are decided in 64 bits where fp32 cannot tell two neighbours apart.  1 <= D <= 16384.
+ * rounding; int8 codes are those of the fp32 quotient y / scale, e4m3 codes those of the exact one (decided in 64 bits
+ * where fp32 cannot tell two neighbours apart).  1 <= D <= 16384.
  * int8 codes and scales are what b200w4a4_gemm and b200w4a4_linear_w4_group take.
  * A row that is not finite, whose mean(s^2) + eps is below fp32's normal range (and not a row of zeros with
  * eps > 0), or whose scale has no normal reciprocal gets scale NaN and codes 0. */
@@ -46,7 +47,8 @@ int b200w4a4_quantize_weight_grouped(const void* w, int w_dtype, void* packed, v
  * for few tokens (the weight is read once per 8 to 32 of them).  x [M, K] contiguous: F16 or BF16
  * (act_scale NULL), or int8 when x_dtype is B200W4A4_X_INT8 (act_scale fp32 [M]).  packed and
  * scale as b200w4a4_quantize_weight_grouped writes them.  out [M, N] and bias [N] (or NULL) are of
- * out_dtype (F16 or BF16); with out_dtype | B200W4A4_BIAS_F32 the bias is fp32 and added as it is.  Products are exact, sums are fp32 (int32 within a group for int8).
+ * out_dtype (F16 or BF16); with out_dtype | B200W4A4_BIAS_F32 the bias is fp32 and added as it is.  Products are
+ * exact, sums are fp32 (int32 within a group for int8).
  * M <= 524280, N <= 2^31 - 512, K <= 1048576. */
 #define B200W4A4_X_INT8 3
 #define B200W4A4_BIAS_F32 16
@@ -78,7 +80,8 @@ size_t b200w4a4_window_attention_workspace_bytes(int B, int Lq, int Lk, int q_he
  * 0..Lk).  Query i of a sequence is at position p = kv_len - Lq + i and sees keys j <= p with
  * j > p - window or j < sinks.  out [B, Lq, q_heads, head_dim] contiguous; lse fp32 [B, q_heads, Lq] or
  * NULL (natural log; what b200w4a4_attn_merge takes).  A query that sees nothing: out 0, lse -inf.
- * Keys that no query can see may hold anything.  window >= 1, sinks >= 0, scale > 0.
+ * Keys that no query can see may hold anything; a value that is not finite reaches only the queries that see its key.
+ * The softmax weights are rounded to dtype for their product with v, all else is fp32.  window >= 1, sinks >= 0, scale > 0.
  * workspace: of the size above, 16-byte aligned, not shared by calls that may overlap.
  * Calls with 128 queries or more wait on barriers inside the kernel, each for at most a second; one that runs out
  * leaves 106 in the device status word (b200w4a4_last_device_status), and rows of out unwritten. */
